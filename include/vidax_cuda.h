@@ -393,6 +393,93 @@ int vx_ln_modulate(const float* x, void* y, const float* w, const float* b, cons
 int vx_gated_residual(float* x, const void* y, const float* gate, int64_t rows, int32_t dim,
                       int32_t rows_per_batch, vx_stream_t stream);
 
+/* ----------------------------------------------------------------------
+ * The 8-bit linear layers of a DiT block (no counterpart in vidax, whose
+ * layers compute in bf16: an inference option of this library around the
+ * Dense layers of WanDiTBlock, src/vidax/models/wan/wan2_1/dit.py:78-156).
+ *
+ * An e4m3 matrix (rows, dim) carries a float32 scale for each block of 128
+ * features of a row (activations) or of 128 rows x 128 features (weights);
+ * the last blocks may be short. Its values are q * s with
+ *   a = max(largest magnitude of the block, 2^-100),  s = a / 448,
+ *   q = e4m3(x * (448 / a)), round to nearest even.
+ * A NaN stays a NaN in its place; a block with an infinity gets s = inf and
+ * stands for NaN. Scales are addressed by two element strides, {row (block),
+ * feature block}; the kernels prefer row stride 1. Rows are addressed by an
+ * element stride; nothing behind a row's `dim` elements is read or written.
+ */
+enum { VX_TYPE_FLOAT = 0, VX_TYPE_BF16 = 1, VX_TYPE_E4M3 = 2 };
+enum { VX_NORM_RMS = 0, VX_NORM_LAYER = 1 };
+enum { VX_ACT_NONE = 0, VX_ACT_GELU_TANH = 1 };
+
+/* vx_quantize_fp8: a float or bf16 matrix as an e4m3 one. */
+typedef struct vx_quantize_fp8_args {
+  const void* src;
+  void* dst;
+  float* scale;
+  int64_t src_stride, dst_stride; /* elements between rows */
+  int64_t scale_stride[2];
+  int64_t rows;
+  int32_t dim;
+  int32_t src_type;               /* VX_TYPE_FLOAT or VX_TYPE_BF16 */
+  int32_t block_rows;             /* 1 (activations) or 128 (weights) */
+} vx_quantize_fp8_args;
+int vx_quantize_fp8(const vx_quantize_fp8_args* args, vx_stream_t stream);
+
+/* vx_add_norm: the gated residual addition, the norm of the sum, modulation
+ * and rounding in one pass (vx_gated_residual followed by vx_ln_modulate and
+ * vx_quantize_fp8, and their RMSNorm forms):
+ *   h = x + float(y) * gate[batch]           (y NULL: h = x, nothing is stored at sum)
+ *   n = (h - m) / sqrt(mean((h - m)^2) + eps) * weight + bias,  m = 0 (RMS), mean(h) (layer)
+ *   out = n * (1 + scale[batch]) + shift[batch]
+ * h is rounded to x's type, stored at `sum` (which may be x) and normalised as
+ * stored. gate, weight, bias, scale and shift are each optional (NULL). */
+typedef struct vx_add_norm_args {
+  const void* x;        /* (rows, dim) x_type */
+  const void* y;        /* (rows, dim) bf16 or NULL */
+  void* sum;            /* (rows, dim) x_type; NULL without y */
+  const float* gate;    /* (rows / rows_per_batch, dim) */
+  const float* weight;  /* (dim) */
+  const float* bias;    /* (dim) */
+  const float* scale;   /* (rows / rows_per_batch, dim) */
+  const float* shift;   /* (rows / rows_per_batch, dim) */
+  void* out;            /* (rows, dim) out_type */
+  float* out_scale;     /* out_type VX_TYPE_E4M3 only: (rows, ceil(dim / 128)) */
+  int64_t x_stride, y_stride, sum_stride, out_stride;  /* elements between rows */
+  int64_t gate_stride, scale_stride, shift_stride;     /* floats between batch items */
+  int64_t out_scale_stride[2];
+  int64_t rows, rows_per_batch;
+  int32_t dim;
+  int32_t x_type;       /* VX_TYPE_FLOAT or VX_TYPE_BF16 */
+  int32_t out_type;     /* VX_TYPE_BF16 or VX_TYPE_E4M3 */
+  int32_t norm;         /* VX_NORM_RMS or VX_NORM_LAYER */
+  float eps;
+} vx_add_norm_args;
+int vx_add_norm(const vx_add_norm_args* args, vx_stream_t stream);
+
+/* vx_linear_fp8: out = act(x w^T + bias) of e4m3 x (m, k), one scale per row
+ * and 128 features, and e4m3 w (n, k), one scale per 128 x 128 block; float32
+ * sums; out bf16, float, or e4m3 with a scale per row and 128 columns. x and w
+ * start, and their rows lie, on 16-byte boundaries. `variant` 0 picks the
+ * kernel by the sizes; 1..4 force a tile (256 x 256 and 256 x 128 on CTA
+ * pairs, 128 x 128, 128 x 64), for tuning. */
+typedef struct vx_linear_fp8_args {
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const float* bias;      /* (n) or NULL */
+  void* out;
+  float* out_scale;       /* out_type VX_TYPE_E4M3 only: (m, ceil(n / 128)) */
+  int64_t x_stride, w_stride, out_stride;  /* elements between rows */
+  int64_t x_scale_stride[2], w_scale_stride[2], out_scale_stride[2];
+  int32_t m, n, k;
+  int32_t out_type;
+  int32_t activation;
+  int32_t variant;
+} vx_linear_fp8_args;
+int vx_linear_fp8(const vx_linear_fp8_args* args, vx_stream_t stream);
+
 /* Self-test of the bounded-wait machinery (failure detection without a GPU
  * fault): runs one CTA that waits on an mbarrier nothing arrives on, through
  * the same bounded wait the kernels use, with a limit of `limit_cycles` SM

@@ -1,0 +1,153 @@
+"""The 8-bit operators without a GPU: the oracle's e4m3 against torch's, and
+every refusal, in Python and at the C ABI (which checks its arguments before
+it touches a device)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp8_ref
+
+
+def test_oracle_e4m3_is_the_format():
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    v = codes[np.isfinite(codes)]
+    assert np.array_equal(fp8_ref.e4m3(v), v)
+    x = np.concatenate([np.random.default_rng(0).standard_normal(20000) * 60,
+                        np.linspace(-0.05, 0.05, 4001), (v[:-1] + v[1:]) / 2])
+    x = x[np.abs(x) <= 448]
+    ref = torch.from_numpy(x.astype(np.float32)).to(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(fp8_ref.e4m3(x.astype(np.float32)), ref)
+
+
+def test_oracle_quantize_round_trip():
+    x = np.random.default_rng(1).standard_normal((5, 300))
+    for r in (1, 128):
+        q, s = fp8_ref.quantize(x, r)
+        back = q * fp8_ref.expand(s, r, 5, 300)
+        assert (np.abs(back - x) <= 2.0 ** -4 * np.abs(x) + 2.0 ** -10 * s.max()).all()
+
+
+def test_fp8_tensor_dequantize():
+    from vidax_b200 import Fp8Tensor
+    d = torch.ones((130, 200)).to(torch.float8_e4m3fn)
+    row = Fp8Tensor(d, torch.arange(260, dtype=torch.float32).view(130, 2)).dequantize()
+    assert row[3, 5] == 6 and row[3, 199] == 7
+    blk = Fp8Tensor(d, torch.arange(4, dtype=torch.float32).view(2, 2)).dequantize()
+    assert blk[127, 127] == 0 and blk[127, 128] == 1 and blk[128, 0] == 2 and blk[129, 199] == 3
+
+
+def test_row_strides():
+    from vidax_b200.fp8 import _empty_fp8, _row_stride
+    t = torch.zeros((3, 4, 32))
+    assert _row_stride(t) == 32 and _row_stride(t[..., :20]) == 32 and _row_stride(t[:, 1:2]) == 128
+    assert _row_stride(t[:, :3]) is None          # a gap between batch items
+    assert _row_stride(t.transpose(0, 1)) is None
+    assert _row_stride(t[..., ::2]) is None
+    assert _row_stride(torch.zeros((1, 32)).expand(4, 32)) is None  # rows that lie on one another
+    assert _row_stride(t[0, 0]) == 32
+    q = _empty_fp8((2, 5, 130), "cpu")
+    assert q.data.shape == (2, 5, 130) and _row_stride(q.data) == 144
+    assert q.scale.shape == (2, 5, 2) and q.scale.flatten(0, 1).stride() == (1, 12)
+
+
+def test_python_refusals():
+    import vidax_b200 as vx
+    f32, bf = torch.zeros((4, 8)), torch.zeros((4, 8), dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        vx.quantize_fp8([1.0])
+    with pytest.raises(NotImplementedError):
+        vx.quantize_fp8(f32.half())
+    with pytest.raises(ValueError, match="CUDA"):
+        vx.quantize_fp8(f32)
+    with pytest.raises(ValueError, match="CUDA"):
+        vx.add_norm(f32, bf)
+    with pytest.raises(NotImplementedError):
+        vx.add_norm(f32.double())
+    q = vx.Fp8Tensor(f32.to(torch.float8_e4m3fn), torch.ones((4, 1)))
+    with pytest.raises(TypeError):
+        vx.linear_fp8(f32, q)
+    with pytest.raises(NotImplementedError):
+        vx.linear_fp8(vx.Fp8Tensor(f32, q.scale), q)
+    with pytest.raises(ValueError, match="CUDA"):
+        vx.linear_fp8(q, q)
+
+
+def _args(cls, **kw):
+    a = cls()
+    for k, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(a, k)[:] = v
+        else:
+            setattr(a, k, v)
+    return a
+
+
+P = 1 << 20  # an aligned address that no refused call reads
+
+
+def _rc(name, a):
+    from vidax_b200 import _lib, fp8
+    rc = fp8._entry(name, a)(ctypes.byref(a), None)
+    return rc, _lib.load().vx_last_error().decode()
+
+
+QOK = dict(src=P, dst=P, scale=P, src_stride=200, dst_stride=208, scale_stride=(1, 4), rows=4, dim=200,
+           src_type=1, block_rows=1)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(rows=-1), 1), (dict(dim=0), 1), (dict(src_type=2), 2), (dict(src_type=7), 2),
+    (dict(block_rows=64), 2), (dict(src=None), 1), (dict(dst=None), 1), (dict(scale=None), 1),
+    (dict(src=P + 1), 1), (dict(scale=P + 2), 1), (dict(src_stride=199), 1), (dict(dst_stride=-8), 1),
+    (dict(scale_stride=(-1, 1)), 1), (dict(rows=1 << 40, src_stride=200), 2)])
+def test_quantize_c_refusals(change, code):
+    from vidax_b200 import fp8
+    rc, msg = _rc("vx_quantize_fp8", _args(fp8.QuantizeFp8Args, **{**QOK, **change}))
+    assert rc == code and msg
+
+
+NOK = dict(x=P, y=P, sum=P, out=P, out_scale=P, x_stride=96, y_stride=96, sum_stride=96, out_stride=96,
+           out_scale_stride=(1, 4), rows=4, rows_per_batch=2, dim=96, x_type=0, out_type=2, norm=0,
+           eps=1e-6)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(rows=-2), 1), (dict(dim=0), 1), (dict(rows_per_batch=0), 1), (dict(rows_per_batch=3), 1),
+    (dict(x_type=2), 2), (dict(out_type=0), 2), (dict(norm=2), 2), (dict(eps=-1.0), 1),
+    (dict(eps=float("nan")), 1), (dict(y=None, gate=P), 1), (dict(x=None), 1), (dict(sum=None), 1),
+    (dict(out=None), 1), (dict(out_scale=None), 1), (dict(x_stride=95), 1), (dict(y=P + 1), 1),
+    (dict(weight=P + 2), 1), (dict(gate=P, gate_stride=-1), 1)])
+def test_add_norm_c_refusals(change, code):
+    from vidax_b200 import fp8
+    rc, msg = _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, **change}))
+    assert rc == code and msg
+
+
+LOK = dict(x=P, x_scale=P, w=P, w_scale=P, out=P, out_scale=P, x_stride=96, w_stride=96, out_stride=64,
+           x_scale_stride=(1, 4), w_scale_stride=(1, 1), out_scale_stride=(1, 4), m=4, n=64, k=96,
+           out_type=1)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(m=-1), 1), (dict(n=0), 1), (dict(k=0), 1), (dict(out_type=3), 2), (dict(activation=2), 2),
+    (dict(variant=-1), 1), (dict(variant=99), 1), (dict(x=None), 1), (dict(w=None), 1),
+    (dict(out=None), 1), (dict(x_scale=None), 1), (dict(w_scale=None), 1),
+    (dict(out_type=2, out_scale=None), 1), (dict(x=P + 8), 1), (dict(w_stride=100), 1),
+    (dict(x_stride=80), 1), (dict(out_stride=63), 1), (dict(bias=P + 1), 1),
+    (dict(w_scale_stride=(1, -1)), 1)])
+def test_linear_c_refusals(change, code):
+    from vidax_b200 import fp8
+    rc, msg = _rc("vx_linear_fp8", _args(fp8.LinearFp8Args, **{**LOK, **change}))
+    assert rc == code and msg
+
+
+def test_c_null_and_empty_calls():
+    from vidax_b200 import _lib, fp8
+    lib = _lib.load()
+    for name in ("vx_quantize_fp8", "vx_add_norm", "vx_linear_fp8"):
+        assert getattr(lib, name)(None, None) == _lib.VX_EINVAL
+    assert _rc("vx_quantize_fp8", _args(fp8.QuantizeFp8Args, **{**QOK, "rows": 0}))[0] == 0
+    assert _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, "rows": 0}))[0] == 0
+    assert _rc("vx_linear_fp8", _args(fp8.LinearFp8Args, **{**LOK, "m": 0}))[0] == 0

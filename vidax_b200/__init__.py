@@ -8,6 +8,10 @@ tensors):
     sequence_parallel_self_attention, sequence_parallel_joint_self_attention,
     neighborhood_attention_3d
 
+and, beside them, the 8-bit linear layers of a DiT block:
+
+    quantize_fp8, add_norm, linear_fp8
+
 Mesh axes (vidax's `sp` axis inside shard_map) bind to torch.distributed
 process groups with `register_axis(name, group)`.
 """
@@ -17,6 +21,13 @@ from .attention import (  # noqa: F401
     dot_product_attention,
     flash_attention,
     local_attention,
+)
+from .fp8 import (  # noqa: F401
+    Fp8Tensor,
+    add_norm,
+    linear_fp8,
+    linear_fp8_flops,
+    quantize_fp8,
 )
 from .hostio import attention_from_host  # noqa: F401
 from .neighborhood import (  # noqa: F401

@@ -36,6 +36,9 @@ EXPORTED_SYMBOLS = (
     "vx_norm_rope_pack",
     "vx_ln_modulate",
     "vx_gated_residual",
+    "vx_quantize_fp8",
+    "vx_add_norm",
+    "vx_linear_fp8",
     "vx_memcpy_rows_async",
     "vx_selftest_wait_timeout",
     "vx_comm_get_unique_id",

@@ -1,0 +1,490 @@
+// Matrix product of e4m3 activations and weights with a float32 scale for
+// each 128 features (activations: per row; weights: per 128 output features):
+//
+//   y[m, n] = act( sum_b xs[m, b] ws[n / 128, b] * S_b[m, n]  +  bias[n] )
+//   S_b[m, n] = sum over the 128 features k of block b of xq[m, k] wq[n, k]
+//
+// S_b is an exact-input tensor-core product (tcgen05 kind::f8f6f4, float32
+// accumulator in TMEM); the scales differ from block to block, so each S_b
+// leaves TMEM and is added to a float32 sum in registers. The tensor core
+// works on the next blocks meanwhile: TMEM holds 512 / kBN block products.
+//
+// CTA roles (320 threads): warps 0-3 and 4-7 are two warpgroups that add up
+// the left and right half of the tile's columns (thread = row), warp 8 feeds
+// shared memory by TMA, warp 9 allocates TMEM and issues the MMAs. CTAs are
+// persistent: each strides over the output tiles, and the three roles' barrier
+// phases run on across tiles, so the next tile's loads and products start
+// while the last one is rounded and stored.
+//
+// kCG = 2 pairs two CTAs (cta_group::2) on one 256-row tile: each holds its
+// 128 rows of the activations and half the tile's weight rows, which halves
+// the weight bytes per CTA (32 KB of operands per 128 x 256 x 128 product
+// instead of 48 KB, what L2 can deliver at the e4m3 rate).
+#pragma once
+
+#include "fp8_common.cuh"
+
+namespace vx {
+namespace fp8 {
+
+enum : int { kOutBf16 = 0, kOutFloat = 1, kOutE4m3 = 2 };
+enum : int { kActNone = 0, kActGeluTanh = 1 };
+
+struct LinearParams {
+  const float* xs;
+  long long xs_rs, xs_bs;       // elements between rows / feature blocks
+  const float* ws;
+  long long ws_rs, ws_bs;       // elements between row blocks / feature blocks
+  const float* bias;            // (n) or NULL
+  void* out;
+  long long out_stride;         // elements between rows
+  float* out_scale;             // e4m3 output only
+  long long os_rs, os_bs;
+  int m, n, kblocks;
+  int tiles_m, tiles_n, tiles;
+  int act;
+  int vec_out;                  // rows of the output start on 32-byte boundaries
+  int* status;
+};
+
+constexpr int kLinThreads = 320;
+constexpr int kLinRows = 128;          // activation rows per CTA
+constexpr int kGroupM = 8;             // row tiles that share a pass over the weights
+
+template <int kCG, int kBN>
+struct LinDims {
+  static constexpr uint32_t kABytes = kLinRows * kBlock;
+  static constexpr uint32_t kBBytes = kBN / kCG * kBlock;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 196608 / kStageBytes < 8 ? 196608 / kStageBytes : 8;
+  static constexpr int kBufs = 512 / kBN < 4 ? 512 / kBN : 4;  // block products in TMEM
+  static constexpr uint32_t kCtl = kStages * kStageBytes;
+  static constexpr uint32_t kAmax = kCtl + 512;                // 2 tiles x 256 floats
+  static constexpr uint32_t kSmemBytes = kAmax + 2048 + 1024;  // + alignment
+};
+
+// control block: barriers, then the TMEM address and the abort flag
+enum : int {
+  kLinFull = 0,        // stages: operands landed (kCG = 2: both CTAs', at the leader)
+  kLinEmpty = 8,       // stages: their MMAs are done
+  kLinAccFull = 16,    // 4: block product complete in TMEM
+  kLinAccEmpty = 20,   // 4: read by every adding warp (kCG = 2: both CTAs', at the leader)
+  kLinAmax = 24,       // both warpgroups' largest magnitudes are written
+  kLinDrain = 25,
+  kLinBars = 26,
+};
+
+// Position in a ring of N barriers and the phase parity of its current round.
+template <int N>
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+
+// 2-D tiled load into this CTA's shared memory; the bytes are counted on `bar`
+// (kCG = 2: the leader CTA's barrier).
+template <int kCG>
+__device__ __forceinline__ void lin_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x,
+                                         int y, uint64_t policy) {
+  if constexpr (kCG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+        : "memory");
+  }
+}
+
+template <int kCG>
+__device__ __forceinline__ void lin_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if constexpr (kCG == 1) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Arrives on `bar` (kCG = 2: at the same offset in both CTAs) when the MMAs
+// issued so far are complete.
+template <int kCG>
+__device__ __forceinline__ void lin_commit(uint32_t bar) {
+  if constexpr (kCG == 1) {
+    tc_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  }
+}
+
+template <int kCG>
+__device__ __forceinline__ void lin_tmem_alloc(uint32_t slot) {
+  if constexpr (kCG == 1) {
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int kCG>
+__device__ __forceinline__ void lin_tmem_dealloc(uint32_t tmem) {
+  if constexpr (kCG == 1) {
+    tmem_dealloc(tmem, 512);
+  } else {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// kind::f8f6f4 instruction descriptor: e4m3 operands (format 0), K-major,
+// float32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// x / (1 + exp(-2 u)) = 0.5 x (1 + tanh u), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// The exponent is bounded so that the product of two denominators stays
+// finite: past 2^60 the quotient is below x * 2^-60, as good as 0.
+__device__ __forceinline__ float gelu_exp(float x) {
+  constexpr float kA = -2.f * 0.7978845608028654f * 1.4426950408889634f;
+  const float t = x * fmaf(kA * 0.044715f * x, x, kA);
+  return ex2_approx(fminf(t, 60.f)) + 1.f;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two elements share one reciprocal: 1/a = b / (a b).
+__device__ __forceinline__ void gelu_tanh2(float& x, float& y) {
+  const float a = gelu_exp(x), b = gelu_exp(y);
+  const float r = rcp_approx(a * b);
+  x *= r * b;
+  y *= r * a;
+}
+
+// Output tile -> (row tile, column tile): kGroupM row tiles run down before
+// the column advances, so the CTAs at work at one time share both operands
+// through L2.
+__device__ __forceinline__ void lin_tile(const LinearParams& p, int t, int& tm, int& tn) {
+  const int per = kGroupM * p.tiles_n;
+  const int g = t / per;
+  const int r = t - g * per;
+  const int gm = min(kGroupM, p.tiles_m - g * kGroupM);
+  tn = r / gm;
+  tm = g * kGroupM + (r - tn * gm);
+}
+
+template <int kCG, int kBN, int kOut>
+__global__ void __launch_bounds__(kLinThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ LinearParams p) {
+  using Dm = LinDims<kCG, kBN>;
+  constexpr int S = Dm::kStages, kBufs = Dm::kBufs;
+  constexpr int kCols = kBN / 2;  // columns of a warpgroup
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) -> uint32_t { return sbase + Dm::kCtl + 8u * i; };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Dm::kCtl + 8 * kLinBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Dm::kCtl + 8 * kLinBars + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kCG == 2 ? cluster_rank() : 0u;
+  const int unit0 = blockIdx.x / kCG, unit_step = gridDim.x / kCG;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(bar(kLinFull + i), 1);
+      mbar_init(bar(kLinEmpty + i), 1);
+    }
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(bar(kLinAccFull + i), 1);
+      mbar_init(bar(kLinAccEmpty + i), 8 * kCG);
+    }
+    mbar_init(bar(kLinAmax), 256);
+    mbar_init(bar(kLinDrain), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) lin_tmem_alloc<kCG>(sbase + Dm::kCtl + 8 * kLinBars);
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (kCG == 2) cluster_sync();  // the peer's barriers exist before anything arrives there
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint64_t policy = l2_policy_evict_last();
+      Ring<S> st;
+      int filled = 0;  // stages that have been loaded at least once
+      bool ok = true;
+      for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+        int tm, tn;
+        lin_tile(p, t, tm, tn);
+        const int row = (tm * kCG + rank) * kLinRows;
+        const int col = tn * kBN + rank * (kBN / kCG);
+        for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
+          const int s = st.i;
+          if (!mbar_wait(bar(kLinEmpty + s), st.phase ^ 1u, abort_flag, p.status,
+                         kDevTimeoutLoad)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = kCG == 2 ? map_to_rank(bar(kLinFull + s), 0) : bar(kLinFull + s);
+          if (rank == 0) mbar_expect_tx(bar(kLinFull + s), kCG * Dm::kStageBytes);
+          const uint32_t dst = sbase + s * Dm::kStageBytes;
+          lin_load<kCG>(dst, &tm_x, full, kb * kBlock, row, policy);
+          lin_load<kCG>(dst + Dm::kABytes, &tm_w, full, kb * kBlock, col, policy);
+          if (filled < S) ++filled;
+        }
+      }
+      if (!ok && rank == 0) {
+        // the loads in flight land before the CTA (pair) gives its memory back
+        for (int i = 0; i < filled; ++i) {
+          st.i = st.i == 0 ? S - 1 : st.i - 1;
+          if (st.i == S - 1) st.phase ^= 1u;
+          mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows * kCG, kBN);
+      Ring<S> st;
+      Ring<kBufs> ac;
+      bool ok = true;
+      for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+        for (int kb = 0; kb < p.kblocks; ++kb, st.next(), ac.next()) {
+          const int s = st.i, a = ac.i;
+          if (!mbar_wait(bar(kLinAccEmpty + a), ac.phase ^ 1u, abort_flag, p.status,
+                         kDevTimeoutMma) ||
+              !mbar_wait(bar(kLinFull + s), st.phase, abort_flag, p.status, kDevTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = sbase + s * Dm::kStageBytes;
+          const uint64_t da = sdesc_sw128(base, 16, 1024);
+          const uint64_t db = sdesc_sw128(base + Dm::kABytes, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
+            lin_mma<kCG>(tmem + a * kBN, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
+          lin_commit<kCG>(bar(kLinEmpty + s));
+          lin_commit<kCG>(bar(kLinAccFull + a));
+        }
+      }
+      if (!ok) {
+        lin_commit<kCG>(bar(kLinDrain));
+        mbar_wait_drain(bar(kLinDrain), 0, p.status);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ sums and output
+    const int wg = warp >> 2;
+    const int r_in = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + wg * kCols;
+    float* amax_s = reinterpret_cast<float*>(smem + Dm::kAmax);
+    const uint32_t empty0 =
+        kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
+    Ring<kBufs> ac;
+    uint32_t tile_parity = 0;
+    bool ok = true;
+    for (int t = unit0; ok && t < p.tiles; t += unit_step, tile_parity ^= 1u) {
+      int tm, tn;
+      lin_tile(p, t, tm, tn);
+      const int row = (tm * kCG + rank) * kLinRows + r_in;
+      const int col = tn * kBN + wg * kCols;
+      const bool live = row < p.m;
+      const float* xs = p.xs + (live ? row * p.xs_rs : 0);
+      const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
+      float acc[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+      // scales two blocks ahead of their use
+      float x0 = xs[0], w0 = ws[0];
+      float x1 = xs[p.kblocks > 1 ? p.xs_bs : 0], w1 = ws[p.kblocks > 1 ? p.ws_bs : 0];
+      for (int kb = 0; kb < p.kblocks; ++kb, ac.next()) {
+        const float sc = x0 * w0;
+        x0 = x1;
+        w0 = w1;
+        const int nxt = min(kb + 2, p.kblocks - 1);
+        x1 = xs[nxt * p.xs_bs];
+        w1 = ws[nxt * p.ws_bs];
+        const int a = ac.i;
+        // the warp leaves together: the loads below need all of its lanes
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag, p.status,
+                                               kDevTimeoutSoftmax))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t sc2 = f2_pack(sc, sc);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(t_lane + a * kBN + c, r);
+          tmem_wait_ld(r);
+          if (c + 32 == kCols) {  // read out: the buffer may take the next product
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (kCG == 2) mbar_arrive_cluster(empty0 + 8u * a);
+              else mbar_arrive(empty0 + 8u * a);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint64_t v = f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                      sc2, f2_pack(acc[c + j], acc[c + j + 1]));
+            f2_unpack(v, acc[c + j], acc[c + j + 1]);
+          }
+        }
+      }
+      if (!ok) break;
+      // ---- bias, activation, rounding, store
+      const int have = p.n - col;  // columns of this warpgroup that exist
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+          if (j < have) acc[j] += __ldg(p.bias + col + j);
+      }
+      if (p.act == kActGeluTanh) {
+#pragma unroll
+        for (int j = 0; j < kCols; j += 2) gelu_tanh2(acc[j], acc[j + 1]);
+      }
+      if constexpr (kOut == kOutE4m3) {
+        float am = 0.f;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) am = fmaxf(am, fabsf(acc[j]));
+        if constexpr (kCols < kBlock) {  // the block's other columns are the other warpgroup's
+          // Two copies by tile parity: a copy is written again only after the
+          // next tile's barrier, which every reader of this one has passed.
+          volatile float* mine = amax_s + tile_parity * 256;
+          mine[wg * 128 + r_in] = am;
+          mbar_arrive(bar(kLinAmax));
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status,
+                                                 kDevTimeoutSoftmax))) {
+            ok = false;
+            break;
+          }
+          am = fmaxf(am, mine[(wg ^ 1) * 128 + r_in]);
+        }
+        float inv;
+        const float s = block_scale(am, inv);
+        if (live && have > 0) {
+          if (col % kBlock == 0)
+            p.out_scale[row * p.os_rs + static_cast<long long>(col / kBlock) * p.os_bs] = s;
+          uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.out_stride + col;
+          if (p.vec_out && have >= kCols) {
+#pragma unroll
+            for (int j = 0; j < kCols; j += 32) {
+              uint32_t q[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                q[i] = pack_e4m3x4(acc[j + 4 * i] * inv, acc[j + 4 * i + 1] * inv,
+                                   acc[j + 4 * i + 2] * inv, acc[j + 4 * i + 3] * inv);
+              st_global_v8(o + j, q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+              if (j < have) o[j] = static_cast<uint8_t>(pack_e4m3x4(acc[j] * inv, 0.f, 0.f, 0.f));
+          }
+        }
+      } else if constexpr (kOut == kOutBf16) {
+        if (live && have > 0) {
+          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + col;
+          if (p.vec_out && have >= kCols) {
+#pragma unroll
+            for (int j = 0; j < kCols; j += 16)
+              st_global_v8(o + j, pack_bf16x2(acc[j], acc[j + 1]), pack_bf16x2(acc[j + 2], acc[j + 3]),
+                           pack_bf16x2(acc[j + 4], acc[j + 5]), pack_bf16x2(acc[j + 6], acc[j + 7]),
+                           pack_bf16x2(acc[j + 8], acc[j + 9]), pack_bf16x2(acc[j + 10], acc[j + 11]),
+                           pack_bf16x2(acc[j + 12], acc[j + 13]),
+                           pack_bf16x2(acc[j + 14], acc[j + 15]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+              if (j < have) o[j] = __float2bfloat16(acc[j]);
+          }
+        }
+      } else {
+        if (live && have > 0) {
+          float* o = static_cast<float*>(p.out) + row * p.out_stride + col;
+          if (p.vec_out && have >= kCols) {
+#pragma unroll
+            for (int j = 0; j < kCols; j += 8)
+              st_global_v8(o + j, __float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
+                           __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]),
+                           __float_as_uint(acc[j + 4]), __float_as_uint(acc[j + 5]),
+                           __float_as_uint(acc[j + 6]), __float_as_uint(acc[j + 7]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+              if (j < have) o[j] = acc[j];
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  // The peer's MMAs read this CTA's shared memory and its arrivals land here:
+  // both stay until both are done.
+  if constexpr (kCG == 2) cluster_sync();
+  tc_fence_after();
+  if (warp == 9) lin_tmem_dealloc<kCG>(tmem);
+}
+
+}  // namespace fp8
+}  // namespace vx

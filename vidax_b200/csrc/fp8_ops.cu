@@ -1,0 +1,371 @@
+// The 8-bit entry points of include/vidax_cuda.h: argument checks, the choice
+// of a kernel variant by sizes and alignment, launches. Nothing here allocates
+// device memory, and no call leaves state for the next one.
+#include "vidax_cuda.h"
+#include "vx_internal.h"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "add_norm.cuh"
+#include "fp8_linear.cuh"
+#include "fp8_quantize.cuh"
+
+namespace {
+
+using namespace vx::fp8;
+
+template <typename... A>
+int fail(int code, const char* fmt, A... a) {
+  return vx_internal_failf(code, fmt, a...);
+}
+int fail(int code, const char* msg) { return vx_internal_fail(code, msg); }
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int launched(const char* what) {
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? VX_OK : vx_internal_cuda_fail(e, what);
+}
+
+int type_size(int32_t t) { return t == VX_TYPE_FLOAT ? 4 : t == VX_TYPE_BF16 ? 2 : 1; }
+
+// Rows of `dim` elements, `stride` apart, that do not overlap.
+int check_rows(const char* name, const void* p, int64_t stride, int64_t rows, int32_t dim,
+               int elem) {
+  if (p == nullptr) return fail(VX_EINVAL, "%s is NULL", name);
+  if (!aligned(p, elem)) return fail(VX_EINVAL, "%s is not aligned to its element", name);
+  if (stride < 0 || (rows > 1 && stride < dim))
+    return fail(VX_EINVAL, "%s row stride %lld is below the row's %d elements", name,
+                (long long)stride, dim);
+  return VX_OK;
+}
+
+int check_scale(const char* name, const void* p, const int64_t (&st)[2]) {
+  if (p == nullptr) return fail(VX_EINVAL, "%s is NULL", name);
+  if (!aligned(p, 4)) return fail(VX_EINVAL, "%s is not aligned to its element", name);
+  if (st[0] < 0 || st[1] < 0) return fail(VX_EINVAL, "%s has a negative stride", name);
+  return VX_OK;
+}
+
+// A vector of 8 elements starts at each multiple of 8 of every row.
+bool vec8(const void* p, int64_t stride, int elem) {
+  const int64_t bytes = std::min(8 * elem, 16);
+  return aligned(p, bytes) && stride * elem % bytes == 0;
+}
+
+// ------------------------------------------------------------------ add_norm
+
+template <typename T, bool kVec>
+void launch_add_norm(const AddNormParams& p, int sms, cudaStream_t s) {
+  // Warps per row: one while its vectors fit a lane's registers, more for
+  // wide rows, and more where there are too few rows to fill the GPU with one
+  // warp each (a row's latency then counts, not its bandwidth).
+  const int vecs = (p.dim + 7) / 8;
+  auto go = [&](auto kernel, int w) {
+    const long long per = 8 / w;
+    kernel<<<static_cast<unsigned>((p.rows + per - 1) / per), 256, 0, s>>>(p);
+  };
+  const bool few = p.rows < 4LL * sms;
+  if (vecs <= 32) return go(add_norm_kernel<T, 1, 1, kVec>, 1);
+  if (!few) {
+    if (vecs <= 64) return go(add_norm_kernel<T, 1, 2, kVec>, 1);
+    if (vecs <= 128) return go(add_norm_kernel<T, 1, 4, kVec>, 1);
+    if (vecs <= 192) return go(add_norm_kernel<T, 1, 6, kVec>, 1);
+  }
+  if (vecs <= 128) return go(add_norm_kernel<T, 4, 1, kVec>, 4);
+  if (vecs <= 256) return go(add_norm_kernel<T, 4, 2, kVec>, 4);
+  if (vecs <= 512) return go(add_norm_kernel<T, 4, 4, kVec>, 4);
+  if (vecs <= 640) return go(add_norm_kernel<T, 4, 5, kVec>, 4);
+  if (vecs <= 1024) return go(add_norm_kernel<T, 8, 4, kVec>, 8);
+  if (vecs <= 2048) return go(add_norm_kernel<T, 8, 8, kVec>, 8);
+  return go(add_norm_kernel<T, 8, 0, kVec>, 8);
+}
+
+// ------------------------------------------------------------------ linear
+
+struct LinVariant {
+  int cg, bn;
+  const void* fn[3];  // by output type
+  uint32_t smem;
+};
+
+template <int kCG, int kBN>
+LinVariant variant() {
+  return {kCG, kBN,
+          {reinterpret_cast<const void*>(&linear_kernel<kCG, kBN, kOutBf16>),
+           reinterpret_cast<const void*>(&linear_kernel<kCG, kBN, kOutFloat>),
+           // a 128-column block of the e4m3 output lies in one tile
+           kBN >= kBlock ? reinterpret_cast<const void*>(
+                               &linear_kernel<kCG, (kBN >= kBlock ? kBN : kBlock), kOutE4m3>)
+                         : nullptr},
+          LinDims<kCG, kBN>::kSmemBytes};
+}
+
+const LinVariant kVariants[] = {variant<2, 256>(), variant<2, 128>(), variant<1, 128>(),
+                                variant<1, 64>()};
+
+std::mutex g_lin_mu;
+std::map<std::pair<const void*, int>, int> g_lin_clusters;
+
+// CTA groups of a variant that are resident at once (GPCs with an odd SM
+// count leave an SM without a partner).
+int resident_groups(const LinVariant& v, const void* fn, int dev, int sms, int* out) {
+  if (v.cg == 1) {
+    *out = sms;
+    return VX_OK;
+  }
+  std::lock_guard<std::mutex> lk(g_lin_mu);
+  int& n = g_lin_clusters[{fn, dev}];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms / 2 * 2);
+    cfg.blockDim = dim3(kLinThreads);
+    cfg.dynamicSmemBytes = v.smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int got = 0;
+    cudaError_t e = cudaOccupancyMaxActiveClusters(&got, fn, &cfg);
+    if (e != cudaSuccess) return vx_internal_cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+    if (got < 1) return fail(VX_ECUDA, "no cluster of 2 CTAs fits this device");
+    n = got;
+  }
+  *out = n;
+  return VX_OK;
+}
+
+int pick_variant(const vx_linear_fp8_args* a, int sms) {
+  int best = 0;
+  double best_t = 1e30;
+  for (int i = 0; i < 4; ++i) {
+    const LinVariant& v = kVariants[i];
+    if (v.fn[a->out_type == VX_TYPE_E4M3 ? 2 : 0] == nullptr) continue;
+    const long long tiles = ((a->m + v.cg * kLinRows - 1) / (v.cg * kLinRows)) *
+                            static_cast<long long>((a->n + v.bn - 1) / v.bn);
+    const long long groups = sms / v.cg;
+    const double t = static_cast<double>((tiles + groups - 1) / groups) * (v.bn + 64);
+    if (t < best_t) best_t = t, best = i;
+  }
+  return best;
+}
+
+}  // namespace
+
+extern "C" int vx_quantize_fp8(const vx_quantize_fp8_args* a, vx_stream_t stream) {
+  if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
+  if (a->rows < 0 || a->dim < 1)
+    return fail(VX_EINVAL, "bad sizes (rows %lld, dim %d)", (long long)a->rows, a->dim);
+  if (a->src_type != VX_TYPE_FLOAT && a->src_type != VX_TYPE_BF16)
+    return fail(VX_EUNSUPPORTED, "src_type %d (float and bf16 are built)", a->src_type);
+  if (a->block_rows != 1 && a->block_rows != kBlock)
+    return fail(VX_EUNSUPPORTED, "block_rows %d (1 and 128 are built)", a->block_rows);
+  if (a->rows == 0) return VX_OK;
+  const int elem = type_size(a->src_type);
+  int rc;
+  if ((rc = check_rows("src", a->src, a->src_stride, a->rows, a->dim, elem)) != VX_OK) return rc;
+  if ((rc = check_rows("dst", a->dst, a->dst_stride, a->rows, a->dim, 1)) != VX_OK) return rc;
+  if ((rc = check_scale("scale", a->scale, a->scale_stride)) != VX_OK) return rc;
+  QuantizeParams p{};
+  p.src = a->src;
+  p.dst = static_cast<uint8_t*>(a->dst);
+  p.scale = a->scale;
+  p.src_stride = a->src_stride;
+  p.dst_stride = a->dst_stride;
+  p.scale_rs = a->scale_stride[0];
+  p.scale_bs = a->scale_stride[1];
+  p.rows = a->rows;
+  p.dim = a->dim;
+  p.blocks = (a->dim - 1) / kBlock + 1;
+  const int per = a->block_rows == 1 ? kRows : kBlock;
+  const long long items = (a->rows + per - 1) / per * p.blocks;
+  if (items > INT_MAX) return fail(VX_EUNSUPPORTED, "too many blocks (%lld)", items);
+  p.items = static_cast<unsigned>(items);
+  p.vec_scale = p.scale_rs == 1 && p.scale_bs % kRows == 0 && aligned(p.scale, 16);
+  const bool vec = vec8(p.src, p.src_stride, elem) && vec8(p.dst, p.dst_stride, 1);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto rows_kernel, auto tiles_kernel) {
+    if (a->block_rows == 1) rows_kernel<<<(p.items + 15) / 16, 256, 0, s>>>(p);
+    else tiles_kernel<<<p.items, 256, 0, s>>>(p);
+  };
+  if (a->src_type == VX_TYPE_FLOAT) {
+    if (vec) go(quantize_rows_kernel<float, true>, quantize_tiles_kernel<float, true>);
+    else go(quantize_rows_kernel<float, false>, quantize_tiles_kernel<float, false>);
+  } else {
+    if (vec) go(quantize_rows_kernel<__nv_bfloat16, true>, quantize_tiles_kernel<__nv_bfloat16, true>);
+    else go(quantize_rows_kernel<__nv_bfloat16, false>, quantize_tiles_kernel<__nv_bfloat16, false>);
+  }
+  return launched("quantize_fp8 launch");
+}
+
+extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
+  if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
+  if (a->rows < 0 || a->dim < 1 || a->rows_per_batch < 1 || a->rows % a->rows_per_batch != 0)
+    return fail(VX_EINVAL, "bad sizes (rows %lld, dim %d, rows_per_batch %lld)", (long long)a->rows,
+                a->dim, (long long)a->rows_per_batch);
+  if (a->x_type != VX_TYPE_FLOAT && a->x_type != VX_TYPE_BF16)
+    return fail(VX_EUNSUPPORTED, "x_type %d (float and bf16 are built)", a->x_type);
+  if (a->out_type != VX_TYPE_BF16 && a->out_type != VX_TYPE_E4M3)
+    return fail(VX_EUNSUPPORTED, "out_type %d (bf16 and e4m3 are built)", a->out_type);
+  if (a->norm != VX_NORM_RMS && a->norm != VX_NORM_LAYER)
+    return fail(VX_EUNSUPPORTED, "norm %d", a->norm);
+  if (!(a->eps >= 0.f) || !std::isfinite(a->eps))
+    return fail(VX_EINVAL, "eps must be finite and >= 0 (got %g)", (double)a->eps);
+  if (a->y == nullptr && a->gate != nullptr) return fail(VX_EINVAL, "gate without y");
+  if (a->rows == 0) return VX_OK;
+  const int xe = type_size(a->x_type), oe = type_size(a->out_type);
+  int rc;
+  if ((rc = check_rows("x", a->x, a->x_stride, a->rows, a->dim, xe)) != VX_OK) return rc;
+  if ((rc = check_rows("out", a->out, a->out_stride, a->rows, a->dim, oe)) != VX_OK) return rc;
+  bool vec = vec8(a->x, a->x_stride, xe) && vec8(a->out, a->out_stride, oe);
+  if (a->y != nullptr) {
+    if ((rc = check_rows("y", a->y, a->y_stride, a->rows, a->dim, 2)) != VX_OK) return rc;
+    if ((rc = check_rows("sum", a->sum, a->sum_stride, a->rows, a->dim, xe)) != VX_OK) return rc;
+    vec = vec && vec8(a->y, a->y_stride, 2) && vec8(a->sum, a->sum_stride, xe);
+  }
+  const float* vs[5] = {a->gate, a->scale, a->shift, a->weight, a->bias};
+  const int64_t vst[5] = {a->gate_stride, a->scale_stride, a->shift_stride, 0, 0};
+  const char* names[5] = {"gate", "scale", "shift", "weight", "bias"};
+  for (int i = 0; i < 5; ++i) {
+    if (vs[i] == nullptr) continue;
+    if (!aligned(vs[i], 4)) return fail(VX_EINVAL, "%s is not aligned to its element", names[i]);
+    if (vst[i] < 0) return fail(VX_EINVAL, "%s has a negative stride", names[i]);
+    vec = vec && vec8(vs[i], vst[i], 4);
+  }
+  if (a->out_type == VX_TYPE_E4M3 &&
+      (rc = check_scale("out_scale", a->out_scale, a->out_scale_stride)) != VX_OK)
+    return rc;
+  int dev, sms;
+  if ((rc = vx_internal_device(&dev, &sms)) != VX_OK) return rc;
+  if (a->rows > INT_MAX) return fail(VX_EUNSUPPORTED, "too many rows");
+  AddNormParams p{};
+  p.x = a->x;
+  p.sum = a->y != nullptr ? a->sum : nullptr;
+  p.y = static_cast<const __nv_bfloat16*>(a->y);
+  p.gate = a->gate;
+  p.w = a->weight;
+  p.b = a->bias;
+  p.scale = a->scale;
+  p.shift = a->shift;
+  p.out = a->out;
+  p.out_scale = a->out_type == VX_TYPE_E4M3 ? a->out_scale : nullptr;
+  p.x_stride = a->x_stride;
+  p.sum_stride = a->sum_stride;
+  p.y_stride = a->y_stride;
+  p.out_stride = a->out_stride;
+  p.gate_stride = a->gate_stride;
+  p.scale_stride = a->scale_stride;
+  p.shift_stride = a->shift_stride;
+  p.out_scale_rs = a->out_scale_stride[0];
+  p.out_scale_bs = a->out_scale_stride[1];
+  p.rows = a->rows;
+  p.rows_per_batch = a->rows_per_batch;
+  p.dim = a->dim;
+  p.layer = a->norm == VX_NORM_LAYER;
+  p.eps = a->eps;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->x_type == VX_TYPE_FLOAT) {
+    if (vec) launch_add_norm<float, true>(p, sms, s);
+    else launch_add_norm<float, false>(p, sms, s);
+  } else {
+    if (vec) launch_add_norm<__nv_bfloat16, true>(p, sms, s);
+    else launch_add_norm<__nv_bfloat16, false>(p, sms, s);
+  }
+  return launched("add_norm launch");
+}
+
+extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
+  if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
+  if (a->m < 0 || a->n < 1 || a->k < 1)
+    return fail(VX_EINVAL, "bad sizes (m %d, n %d, k %d)", a->m, a->n, a->k);
+  const int out_idx = a->out_type == VX_TYPE_BF16    ? kOutBf16
+                      : a->out_type == VX_TYPE_FLOAT ? kOutFloat
+                      : a->out_type == VX_TYPE_E4M3  ? kOutE4m3
+                                                     : -1;
+  if (out_idx < 0) return fail(VX_EUNSUPPORTED, "out_type %d", a->out_type);
+  if (a->activation != VX_ACT_NONE && a->activation != VX_ACT_GELU_TANH)
+    return fail(VX_EUNSUPPORTED, "activation %d", a->activation);
+  if (a->variant < 0 || a->variant > 4) return fail(VX_EINVAL, "variant %d", a->variant);
+  if (a->m == 0) return VX_OK;
+  int rc;
+  if ((rc = check_rows("x", a->x, a->x_stride, a->m, a->k, 1)) != VX_OK) return rc;
+  if ((rc = check_rows("w", a->w, a->w_stride, a->n, a->k, 1)) != VX_OK) return rc;
+  if ((rc = check_rows("out", a->out, a->out_stride, a->m, a->n, type_size(a->out_type))) != VX_OK)
+    return rc;
+  if (!aligned(a->x, 16) || !aligned(a->w, 16) || a->x_stride % 16 != 0 || a->w_stride % 16 != 0)
+    return fail(VX_EINVAL, "x and w must start, and their rows must lie, on 16-byte boundaries");
+  if ((rc = check_scale("x_scale", a->x_scale, a->x_scale_stride)) != VX_OK) return rc;
+  if ((rc = check_scale("w_scale", a->w_scale, a->w_scale_stride)) != VX_OK) return rc;
+  if (out_idx == kOutE4m3 &&
+      (rc = check_scale("out_scale", a->out_scale, a->out_scale_stride)) != VX_OK)
+    return rc;
+  if (a->bias != nullptr && !aligned(a->bias, 4))
+    return fail(VX_EINVAL, "bias is not aligned to its element");
+  int dev, sms;
+  if ((rc = vx_internal_device(&dev, &sms)) != VX_OK) return rc;
+  const LinVariant& v = kVariants[a->variant > 0 ? a->variant - 1 : pick_variant(a, sms)];
+  const void* fn = v.fn[out_idx];
+  if (fn == nullptr) return fail(VX_EUNSUPPORTED, "this variant has no e4m3 output");
+
+  LinearParams p{};
+  p.xs = a->x_scale;
+  p.xs_rs = a->x_scale_stride[0];
+  p.xs_bs = a->x_scale_stride[1];
+  p.ws = a->w_scale;
+  p.ws_rs = a->w_scale_stride[0];
+  p.ws_bs = a->w_scale_stride[1];
+  p.bias = a->bias;
+  p.out = a->out;
+  p.out_stride = a->out_stride;
+  p.out_scale = a->out_scale;
+  p.os_rs = a->out_scale_stride[0];
+  p.os_bs = a->out_scale_stride[1];
+  p.m = a->m;
+  p.n = a->n;
+  p.kblocks = (a->k - 1) / kBlock + 1;
+  p.tiles_m = (a->m - 1) / (v.cg * kLinRows) + 1;
+  p.tiles_n = (a->n - 1) / v.bn + 1;
+  const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+  if (tiles > INT_MAX / 2 || static_cast<long long>(kGroupM) * p.tiles_n > INT_MAX)
+    return fail(VX_EUNSUPPORTED, "too many output tiles (%lld)", tiles);
+  p.tiles = static_cast<int>(tiles);
+  p.act = a->activation;
+  p.vec_out = aligned(a->out, 32) && a->out_stride * type_size(a->out_type) % 32 == 0;
+  if ((rc = vx_internal_status_word(&p.status)) != VX_OK) return rc;
+
+  // One row needs no stride; the map wants one that is a multiple of 16.
+  const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
+  const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
+  CUtensorMap tx, tw;
+  if ((rc = vx_internal_byte_tmap(&tx, a->x, a->k, a->m, xst, kLinRows)) != VX_OK) return rc;
+  if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, v.bn / v.cg)) != VX_OK) return rc;
+  if ((rc = vx_internal_prepare_kernel(fn, dev, v.smem)) != VX_OK) return rc;
+  int groups;
+  if ((rc = resident_groups(v, fn, dev, sms, &groups)) != VX_OK) return rc;
+
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tiles, groups)) * v.cg);
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = v.smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = v.cg;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  void* args[3] = {&tx, &tw, &p};
+  cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return vx_internal_cuda_fail(e, "linear_fp8 launch");
+  }
+  return VX_OK;
+}

@@ -50,6 +50,17 @@ int cuda_fail(cudaError_t e, const char* what) {
 
 int vx_internal_fail(int code, const char* msg) { return fail(code, "%s", msg); }
 
+int vx_internal_failf(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+
+int vx_internal_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
 // Device status word: kernels OR timeout codes into it (one instance per
 // device context).
 __device__ int g_vx_status;
@@ -164,6 +175,31 @@ int prepare_kernel(const void* fn, int dev, size_t smem) {
 }
 
 }  // namespace
+
+int vx_internal_device(int* dev, int* sms) {
+  int rc = current_device(dev);
+  return rc != VX_OK ? rc : num_sms(*dev, sms);
+}
+
+int vx_internal_prepare_kernel(const void* fn, int dev, size_t smem) {
+  return prepare_kernel(fn, dev, smem);
+}
+
+int vx_internal_byte_tmap(CUtensorMap* tm, const void* base, uint64_t cols, uint64_t rows,
+                          uint64_t stride, uint32_t box_rows) {
+  EncodeTiledFn enc;
+  int rc = get_encode_fn(&enc);
+  if (rc != VX_OK) return rc;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {stride};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t elem_str[2] = {1, 1};
+  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                   elem_str, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VX_EINVAL, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+  return VX_OK;
+}
 
 int vx_internal_status_word(int** out) {
   int dev = 0;

@@ -1,0 +1,390 @@
+"""The 8-bit linear layers of a DiT block on B200.
+
+vidax computes its Dense layers in bf16 (WanDiTBlock, src/vidax/models/wan/
+wan2_1/dit.py:78-156); this module is this library's 8-bit option for them.
+A tensor is held as e4m3 values with a float32 scale for each block of 128
+features (`Fp8Tensor`), and three kernels make and use it:
+
+* `quantize_fp8`  -- a bf16 / float32 tensor as an Fp8Tensor;
+* `add_norm`      -- the gated residual addition, RMSNorm or LayerNorm,
+                     modulation, and the rounding to e4m3 (or bf16) in one
+                     pass over the residual stream;
+* `linear_fp8`    -- x @ w^T on the tensor cores' 8-bit path, with bias and
+                     tanh GELU, its output in bf16, float32 or e4m3 again.
+
+`vidax_b200.wan_dit.quantize_params` gives a whole DiT's weights this form.
+Inference only, like the rest of this package: the outputs carry no gradient.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+_NORMS = {"rms": 0, "layer": 1}
+_ACTS = {None: 0, "gelu_tanh": 1}
+
+
+class QuantizeFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+        ("src_stride", ctypes.c_int64), ("dst_stride", ctypes.c_int64),
+        ("scale_stride", ctypes.c_int64 * 2),
+        ("rows", ctypes.c_int64),
+        ("dim", ctypes.c_int32), ("src_type", ctypes.c_int32), ("block_rows", ctypes.c_int32),
+    ]
+
+
+class AddNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("sum", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_scale", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+        ("sum_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64), ("scale_stride", ctypes.c_int64),
+        ("shift_stride", ctypes.c_int64),
+        ("out_scale_stride", ctypes.c_int64 * 2),
+        ("rows", ctypes.c_int64), ("rows_per_batch", ctypes.c_int64),
+        ("dim", ctypes.c_int32), ("x_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+        ("norm", ctypes.c_int32), ("eps", ctypes.c_float),
+    ]
+
+
+class LinearFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_scale", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+        ("x_scale_stride", ctypes.c_int64 * 2), ("w_scale_stride", ctypes.c_int64 * 2),
+        ("out_scale_stride", ctypes.c_int64 * 2),
+        ("m", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+        ("out_type", ctypes.c_int32), ("activation", ctypes.c_int32), ("variant", ctypes.c_int32),
+    ]
+
+
+class Fp8Tensor(NamedTuple):
+    """e4m3 values with a float32 scale per block of 128 features.
+
+    data:  (..., K) float8_e4m3fn, features contiguous.
+    scale: activations (..., ceil(K / 128)), one scale per row and block;
+           weights (N, K): (ceil(N / 128), ceil(K / 128)), one per 128 x 128
+           block.
+    """
+    data: torch.Tensor
+    scale: torch.Tensor
+
+    def dequantize(self) -> torch.Tensor:
+        """The float32 values this tensor stands for."""
+        k = self.data.shape[-1]
+        s = self.scale.repeat_interleave(BLOCK, dim=-1)[..., :k]
+        if self.scale.shape[:-1] != self.data.shape[:-1]:
+            s = s.repeat_interleave(BLOCK, dim=0)[:self.data.shape[0]]
+        return self.data.float() * s
+
+
+def _entry(name: str, args):
+    fn = getattr(_lib.load(), name)
+    fn.argtypes = [ctypes.POINTER(type(args)), ctypes.c_void_p]
+    fn.restype = ctypes.c_int
+    return fn
+
+
+def _launch(name: str, args, device: torch.device) -> None:
+    fn = _entry(name, args)
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device)
+        _lib.check(fn(ctypes.byref(args), ctypes.c_void_p(stream.cuda_stream)))
+
+
+def _check_cuda(name: str, t, dtypes, min_dim: int = 1) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dim() < min_dim:
+        raise ValueError(f"{name} must have at least {min_dim} dimensions, got shape {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise NotImplementedError(f"{name}.dtype={t.dtype}: the kernel takes "
+                                  + " or ".join(str(d) for d in dtypes))
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this implementation has no CPU path)")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} requires a gradient: this operator is inference only")
+
+
+def _row_stride(t: torch.Tensor) -> Optional[int]:
+    """Elements between the consecutive rows (..., K) -> (rows, K) of `t`
+    without a copy, or None where they are not evenly spaced."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return None
+    dims = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    for (_, s0), (n1, s1) in zip(dims, dims[1:]):
+        if s0 != n1 * s1:
+            return None
+    stride = dims[-1][1] if dims else t.shape[-1]
+    return stride if stride >= t.shape[-1] else None
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """`t` (a copy where its rows are not evenly spaced) and its row stride."""
+    s = _row_stride(t)
+    if s is None:
+        t = t.contiguous()
+        s = t.shape[-1]
+    return t, s
+
+
+def _empty_fp8(shape, device) -> Fp8Tensor:
+    """An activation's storage: rows on 16-byte boundaries (the matrix
+    product's loads need that), the scales of one block of features side by
+    side (a warp of the matrix product reads those of 32 rows at once)."""
+    *lead, k = shape
+    rows = 1
+    for n in lead:
+        rows *= n
+    ld = -(-k // 16) * 16
+    data = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)[:, :k]
+    ls = -(-rows // 4) * 4
+    scale = torch.empty((-(-k // BLOCK), ls), dtype=torch.float32, device=device)[:, :rows].t()
+    if len(lead) == 1:
+        return Fp8Tensor(data, scale)
+    return Fp8Tensor(data.unflatten(0, lead), scale.unflatten(0, lead))
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
+    """x (..., K) bf16 or float32 as e4m3 with float32 scales, one per row and
+    128 features, or with block_rows = 128 (x a weight (N, K)) one per
+    128 x 128 block:
+
+        a = max(largest magnitude of the block, 2^-100)
+        scale = a / 448,   data = e4m3(x * (448 / a)), round to nearest even
+
+    A NaN stays a NaN in its place; a block with an infinity stands for NaN.
+    """
+    _check_cuda("x", x, (torch.bfloat16, torch.float32), 2)
+    if block_rows not in (1, BLOCK):
+        raise NotImplementedError(f"block_rows {block_rows}: 1 and {BLOCK} are built")
+    if block_rows == BLOCK and x.dim() != 2:
+        raise ValueError(f"a weight is (N, K), got {tuple(x.shape)}")
+    if x.shape[-1] < 1:
+        raise ValueError("x has no features")
+    out = _empty_fp8(x.shape, x.device)
+    if block_rows == BLOCK:
+        out = Fp8Tensor(out.data, torch.empty((-(-x.shape[0] // BLOCK), out.scale.shape[-1]),
+                                              dtype=torch.float32, device=x.device))
+    if x.numel() == 0:
+        return out
+    x, stride = _rows(x)
+    a = QuantizeFp8Args()
+    a.src, a.dst, a.scale = x.data_ptr(), out.data.data_ptr(), out.scale.data_ptr()
+    a.src_stride, a.dst_stride = stride, _row_stride(out.data)
+    a.scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
+    a.rows, a.dim = x.numel() // x.shape[-1], x.shape[-1]
+    a.src_type, a.block_rows = _TYPES[x.dtype], block_rows
+    _launch("vx_quantize_fp8", a, x.device)
+    return out
+
+
+def _vector(name: str, t: Optional[torch.Tensor], shape, device):
+    """A float32 vector (dim) or per-batch-item vector (B, dim) / (B, 1, dim)
+    in place (converted where its type or layout differs)."""
+    if t is None:
+        return None, 0
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device != device:
+        raise ValueError(f"{name} must live on x's device")
+    if t.dim() == 3 and len(shape) == 2 and t.shape[1] == 1:
+        t = t[:, 0]
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    t = t.detach().to(torch.float32)
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if len(shape) == 2 and shape[0] > 1 else 0)
+
+
+def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
+             gate: Optional[torch.Tensor] = None, *, norm: str = "rms",
+             weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+             scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
+             eps: float = 1e-6, out_dtype: torch.dtype = torch.bfloat16,
+             residual_out: Optional[torch.Tensor] = None):
+    """The residual addition and the norm that follows it, in one pass:
+
+        h = x + y * gate
+        n = (h - m) / sqrt(mean((h - m)^2) + eps) * weight + bias
+        out = n * (1 + scale) + shift
+
+    with m = 0 (norm="rms") or mean(h) (norm="layer"). x: the residual stream
+    (B, L, dim) or (L, dim), float32 or bf16; y: the sub-layer's output, bf16,
+    or None (h = x). weight / bias: (dim); gate / scale / shift: (B, dim) or
+    (B, 1, dim) ((1, dim) for a 2-D x). Each may be None. h is rounded to x's
+    type and normalised as stored.
+
+    Returns (out, h). out: bf16, or an Fp8Tensor for out_dtype
+    torch.float8_e4m3fn. h: written to `residual_out` where that is given (x
+    itself for an update in place), else to a new tensor; x itself without y.
+    """
+    _check_cuda("x", x, (torch.float32, torch.bfloat16), 2)
+    if x.dim() > 3:
+        raise ValueError(f"x must be (B, L, dim) or (L, dim), got {tuple(x.shape)}")
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    if out_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+        raise NotImplementedError(f"out_dtype {out_dtype}: bfloat16 and float8_e4m3fn are built")
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    dim = x.shape[-1]
+    batch = x.shape[0] if x.dim() == 3 else 1
+    if dim < 1:
+        raise ValueError("x has no features")
+    if y is None:
+        if gate is not None or residual_out is not None:
+            raise ValueError("gate and residual_out belong to y")
+    else:
+        _check_cuda("y", y, (torch.bfloat16,))
+        if y.shape != x.shape or y.device != x.device:
+            raise ValueError(f"y {tuple(y.shape)} must have x's shape {tuple(x.shape)} and device")
+    total = x
+    if y is not None:
+        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None \
+            else residual_out
+        if total.shape != x.shape or total.dtype != x.dtype or total.device != x.device:
+            raise ValueError("residual_out must have x's shape, type and device")
+        if _row_stride(total) is None:
+            raise ValueError("residual_out must have evenly spaced rows of contiguous features")
+        if total.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("residual_out requires a gradient: this operator is inference only")
+    out = _empty_fp8(x.shape, x.device) if out_dtype == torch.float8_e4m3fn \
+        else torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    dev = x.device
+    vecs = {n: _vector(n, t, s, dev) for n, t, s in (
+        ("gate", gate, (batch, dim)), ("scale", scale, (batch, dim)), ("shift", shift, (batch, dim)),
+        ("weight", weight, (dim,)), ("bias", bias, (dim,)))}
+    if x.numel() == 0:
+        return out, total
+    a = AddNormArgs()
+    xr, a.x_stride = _rows(x)
+    a.x = xr.data_ptr()
+    if y is not None:
+        yr, a.y_stride = _rows(y)
+        a.y, a.sum, a.sum_stride = yr.data_ptr(), total.data_ptr(), _row_stride(total)
+    for n, (t, s) in vecs.items():
+        if t is not None:
+            setattr(a, n, t.data_ptr())
+            if n in ("gate", "scale", "shift"):
+                setattr(a, n + "_stride", s)
+    if isinstance(out, Fp8Tensor):
+        a.out, a.out_stride = out.data.data_ptr(), _row_stride(out.data)
+        a.out_scale = out.scale.data_ptr()
+        a.out_scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
+        a.out_type = _TYPES[torch.float8_e4m3fn]
+    else:
+        a.out, a.out_stride, a.out_type = out.data_ptr(), dim, _TYPES[torch.bfloat16]
+    a.rows, a.rows_per_batch = batch * x.shape[-2], x.shape[-2]
+    a.dim, a.x_type, a.norm, a.eps = dim, _TYPES[x.dtype], _NORMS[norm], eps
+    _launch("vx_add_norm", a, dev)
+    return out, total
+
+
+def _fp8_rows(name: str, t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """e4m3 rows on 16-byte boundaries (a padded copy where they are not) and
+    their stride."""
+    s = _row_stride(t)
+    k = t.shape[-1]
+    rows = t.numel() // k
+    if s is not None and t.data_ptr() % 16 == 0 and (s % 16 == 0 or rows == 1):
+        return t, -(-s // 16) * 16
+    ld = -(-k // 16) * 16
+    buf = torch.empty((rows, ld), dtype=torch.uint8, device=t.device)
+    buf[:, :k] = t.reshape(rows, k).view(torch.uint8)
+    return buf, ld
+
+
+def _scale_strides(scale: torch.Tensor):
+    """`scale` (..., blocks) as (rows, blocks) and its two strides."""
+    if scale.dim() > 2:
+        scale = scale.flatten(0, -2)
+    return scale, (scale.stride(0), scale.stride(1))
+
+
+def linear_fp8(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *,
+               activation: Optional[str] = None, out_dtype: torch.dtype = torch.bfloat16,
+               variant: int = 0):
+    """act(x @ w^T + bias) with x (..., K) quantised per row and w (N, K)
+    quantised per 128 x 128 block (`quantize_fp8`), summed in float32:
+
+        y[m, n] = sum_b x.scale[m, b] * w.scale[n // 128, b]
+                        * sum_{k in block b} x.data[m, k] * w.data[n, k]
+
+    bias: (N) or None; activation: None or "gelu_tanh". Returns (..., N) in
+    out_dtype: bfloat16, float32, or (float8_e4m3fn) an Fp8Tensor with a scale
+    per row and 128 columns, the next layer's input. Rows of x or w that do
+    not lie on 16-byte boundaries are copied first; `quantize_fp8` and
+    `add_norm` lay theirs out so. `variant` forces a kernel variant (tuning).
+    """
+    for name, t in (("x", x), ("w", w)):
+        if not isinstance(t, tuple) or len(t) != 2:
+            raise TypeError(f"{name} must be an Fp8Tensor, got {type(t).__name__}")
+    xd, xs = x
+    wd, ws = w
+    _check_cuda("x.data", xd, (torch.float8_e4m3fn,), 2)
+    _check_cuda("w.data", wd, (torch.float8_e4m3fn,), 2)
+    _check_cuda("x.scale", xs, (torch.float32,), 2)
+    _check_cuda("w.scale", ws, (torch.float32,), 2)
+    if wd.dim() != 2 or wd.shape[0] < 1:
+        raise ValueError(f"w.data must be (N, K), got {tuple(wd.shape)}")
+    N, K = wd.shape
+    if K < 1 or xd.shape[-1] != K:
+        raise ValueError(f"x {tuple(xd.shape)} and w {tuple(wd.shape)} disagree on the features")
+    kb = -(-K // BLOCK)
+    if tuple(xs.shape) != (*xd.shape[:-1], kb):
+        raise ValueError(f"x.scale has shape {tuple(xs.shape)}, expected {(*xd.shape[:-1], kb)}")
+    if tuple(ws.shape) != (-(-N // BLOCK), kb):
+        raise ValueError(f"w.scale has shape {tuple(ws.shape)}, expected {(-(-N // BLOCK), kb)}")
+    dev = xd.device
+    if not (dev == xs.device == wd.device == ws.device):
+        raise ValueError("x and w must live on the same device")
+    if activation not in _ACTS:
+        raise NotImplementedError(f"activation {activation!r}: None and 'gelu_tanh' are built")
+    if out_dtype not in _TYPES:
+        raise NotImplementedError(f"out_dtype {out_dtype}: bfloat16, float32 and float8_e4m3fn are built")
+    bias, _ = _vector("bias", bias, (N,), dev)
+    shape = (*xd.shape[:-1], N)
+    out = _empty_fp8(shape, dev) if out_dtype == torch.float8_e4m3fn \
+        else torch.empty(shape, dtype=out_dtype, device=dev)
+    if xd.numel() == 0:
+        return out
+    a = LinearFp8Args()
+    xd, a.x_stride = _fp8_rows("x", xd)
+    wd, a.w_stride = _fp8_rows("w", wd)
+    xs, a.x_scale_stride[:] = _scale_strides(xs)
+    ws, a.w_scale_stride[:] = _scale_strides(ws)
+    a.x, a.w, a.x_scale, a.w_scale = (t.data_ptr() for t in (xd, wd, xs, ws))
+    a.bias = bias.data_ptr() if bias is not None else None
+    if isinstance(out, Fp8Tensor):
+        a.out, a.out_stride = out.data.data_ptr(), _row_stride(out.data)
+        a.out_scale = out.scale.data_ptr()
+        a.out_scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
+    else:
+        a.out, a.out_stride = out.data_ptr(), N
+    m = 1
+    for n in shape[:-1]:
+        m *= n
+    a.m, a.n, a.k = m, N, K
+    a.out_type, a.activation, a.variant = _TYPES[out_dtype], _ACTS[activation], variant
+    _launch("vx_linear_fp8", a, dev)
+    return out
+
+
+def linear_fp8_flops(m: int, n: int, k: int) -> float:
+    """FLOPs of one matrix product, 2*m*n*k."""
+    return 2.0 * m * n * k
