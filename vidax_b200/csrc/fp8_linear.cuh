@@ -9,12 +9,17 @@
 // leaves TMEM and is added to a float32 sum in registers. The tensor core
 // works on the next blocks meanwhile: TMEM holds 512 / kBN block products.
 //
-// CTA roles (320 threads): warps 0-3 and 4-7 are two warpgroups that add up
+// CTA roles (384 threads): warps 0-3 and 4-7 are two warpgroups that add up
 // the left and right half of the tile's columns (thread = row), warp 8 feeds
-// shared memory by TMA, warp 9 allocates TMEM and issues the MMAs. CTAs are
-// persistent: each strides over the output tiles, and the three roles' barrier
-// phases run on across tiles, so the next tile's loads and products start
-// while the last one is rounded and stored.
+// shared memory by TMA, warp 9 allocates TMEM and issues the MMAs, warp 10
+// fetches the scales (cp.async, any strides) as far ahead as warp 8 fetches
+// the operands: read from global memory where they are used, their latency
+// cost a third of the time of a long sum. CTAs are persistent: each strides
+// over the output tiles, and the roles' barrier phases run on across tiles, so
+// the next tile's loads and products start while the last one is rounded and
+// stored. A finished tile leaves through shared memory by TMA (full 128-byte
+// lines, edges clipped by the tensor map); an output that TMA cannot address
+// is stored element by element.
 //
 // kCG = 2 pairs two CTAs (cta_group::2) on one 256-row tile: each holds its
 // 128 rows of the activations and half the tile's weight rows, which halves
@@ -43,24 +48,40 @@ struct LinearParams {
   int m, n, kblocks;
   int tiles_m, tiles_n, tiles;
   int act;
-  int vec_out;                  // rows of the output start on 32-byte boundaries
+  int tma_out;                  // the output goes through tm_o
   int* status;
 };
 
-constexpr int kLinThreads = 320;
+constexpr int kLinThreads = 384;       // 3 warpgroups: two add and store, one feeds
 constexpr int kLinRows = 128;          // activation rows per CTA
 constexpr int kGroupM = 8;             // row tiles that share a pass over the weights
+constexpr int kScaleSlots = 16;        // blocks of scales in shared memory
+constexpr int kScaleFloats = 132;      // 128 rows, 2 warpgroups' weight scales, padding
+// Registers: 384 threads start with 168 each; the feeding warpgroup gives 96
+// of its up and each adding one takes 48 (72 + 2 * 216 = 3 * 168), room for
+// 128 sums and a block product's next columns.
+constexpr int kFeedRegs = 72, kSumRegs = 216;
 
 template <int kCG, int kBN>
 struct LinDims {
   static constexpr uint32_t kABytes = kLinRows * kBlock;
   static constexpr uint32_t kBBytes = kBN / kCG * kBlock;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes < 8 ? 196608 / kStageBytes : 8;
+  static constexpr uint32_t kStoreBytes = 8 * 4096;            // 32 rows x 128 bytes per warp
+  static constexpr uint32_t kRest = kStoreBytes + kScaleSlots * kScaleFloats * 4 + 8 * 512 + 2048 + 512;
+  static constexpr int kFit = (232448 - 1024 - kRest) / kStageBytes;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kBufs = 512 / kBN < 4 ? 512 / kBN : 4;  // block products in TMEM
-  static constexpr uint32_t kCtl = kStages * kStageBytes;
-  static constexpr uint32_t kAmax = kCtl + 512;                // 2 tiles x 256 floats
-  static constexpr uint32_t kSmemBytes = kAmax + 2048 + 1024;  // + alignment
+  // A scale slot is written S blocks ahead of the tensor core, which is at
+  // most kBufs blocks ahead of the sums that read it.
+  static_assert(kStages + kBufs <= kScaleSlots, "scale slots");
+  static constexpr uint32_t kStore = kStages * kStageBytes;
+  static constexpr uint32_t kScales = kStore + kStoreBytes;
+  static constexpr uint32_t kBias = kScales + kScaleSlots * kScaleFloats * 4;  // 128 floats per warp
+  static constexpr uint32_t kAmax = kBias + 8 * 512;           // 2 tiles x 256 floats
+  static constexpr uint32_t kCtl = kAmax + 2048;
+  static constexpr uint32_t kSmemBytes = kCtl + 512 + 1024;    // + alignment
+  static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
 };
 
 // control block: barriers, then the TMEM address and the abort flag
@@ -71,7 +92,8 @@ enum : int {
   kLinAccEmpty = 20,   // 4: read by every adding warp (kCG = 2: both CTAs', at the leader)
   kLinAmax = 24,       // both warpgroups' largest magnitudes are written
   kLinDrain = 25,
-  kLinBars = 26,
+  kLinScale = 26,      // 16: a block's scales landed
+  kLinBars = 42,
 };
 
 // Position in a ring of N barriers and the phase parity of its current round.
@@ -100,8 +122,11 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// Relaxed: what it announces is that TMEM has been read (the reads themselves
+// have completed), not a write. A release at cluster scope would wait for
+// every outstanding global load of the thread (measured: half of all stalls).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                : "memory");
 }
 
@@ -205,6 +230,40 @@ __device__ __forceinline__ void gelu_tanh2(float& x, float& y) {
   y *= r * a;
 }
 
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(there ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void lin_store(const CUtensorMap* tm, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(tm)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+
+// 16 bytes of output: bf16 x 8, float x 4, e4m3 x 16 (already scaled by inv).
+template <int kOut>
+__device__ __forceinline__ void lin_pack16(const float* v, float inv, uint32_t (&q)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kOut == kOutBf16) q[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    else if constexpr (kOut == kOutFloat) q[i] = __float_as_uint(v[i]);
+    else
+      q[i] = pack_e4m3x4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+  }
+}
+
 // Output tile -> (row tile, column tile): kGroupM row tiles run down before
 // the column advances, so the CTAs at work at one time share both operands
 // through L2.
@@ -220,7 +279,7 @@ __device__ __forceinline__ void lin_tile(const LinearParams& p, int t, int& tm, 
 template <int kCG, int kBN, int kOut>
 __global__ void __launch_bounds__(kLinThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                  const __grid_constant__ LinearParams p) {
+                  const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ LinearParams p) {
   using Dm = LinDims<kCG, kBN>;
   constexpr int S = Dm::kStages, kBufs = Dm::kBufs;
   constexpr int kCols = kBN / 2;  // columns of a warpgroup
@@ -244,6 +303,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_init(bar(kLinAccFull + i), 1);
       mbar_init(bar(kLinAccEmpty + i), 8 * kCG);
     }
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(bar(kLinScale + i), 32);
     mbar_init(bar(kLinAmax), 256);
     mbar_init(bar(kLinDrain), 1);
     *abort_flag = 0;
@@ -260,6 +320,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFeedRegs));
   if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -328,15 +390,50 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         mbar_wait_drain(bar(kLinDrain), 0, p.status);
       }
     }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ scales
+    Ring<S> st;
+    Ring<kScaleSlots> sl;
+    bool ok = true;
+    for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+      int tm, tn;
+      lin_tile(p, t, tm, tn);
+      const int row = (tm * kCG + rank) * kLinRows + lane;
+      const int col = tn * kBN + (lane & 1) * kCols;
+      const float* xs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
+      const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
+      for (int kb = 0; kb < p.kblocks; ++kb, st.next(), sl.next()) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinEmpty + st.i), st.phase ^ 1u, abort_flag,
+                                               p.status, kDevTimeoutLoad))) {
+          ok = false;
+          break;
+        }
+        const uint32_t dst = sbase + Dm::kScales + sl.i * (kScaleFloats * 4) + lane * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
+        if (lane < 2) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
+        cp_async_arrive(bar(kLinScale + sl.i));
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
     // ------------------------------------------------------------ sums and output
     const int wg = warp >> 2;
-    const int r_in = (warp & 3) * 32 + lane;
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + wg * kCols;
+    const int r_warp = (warp & 3) * 32;
+    const int r_in = r_warp + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(r_warp) << 16) + wg * kCols;
+    const float* scale_s = reinterpret_cast<const float*>(smem + Dm::kScales);
+    float* bias_s = reinterpret_cast<float*>(smem + Dm::kBias) + warp * 128;
     float* amax_s = reinterpret_cast<float*>(smem + Dm::kAmax);
-    const uint32_t empty0 =
-        kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
+    const uint32_t empty0 = kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
     Ring<kBufs> ac;
+    Ring<kScaleSlots> sl;
     uint32_t tile_parity = 0;
     bool ok = true;
     for (int t = unit0; ok && t < p.tiles; t += unit_step, tile_parity ^= 1u) {
@@ -345,36 +442,37 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       const int row = (tm * kCG + rank) * kLinRows + r_in;
       const int col = tn * kBN + wg * kCols;
       const bool live = row < p.m;
-      const float* xs = p.xs + (live ? row * p.xs_rs : 0);
-      const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
+      const int have = p.n - col;  // columns of this warpgroup that exist
+      float bias[kCols / 32];      // of columns col + lane + 32 i
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i)
+        bias[i] = p.bias != nullptr && lane + 32 * i < have ? p.bias[col + lane + 32 * i] : 0.f;
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-      // scales two blocks ahead of their use
-      float x0 = xs[0], w0 = ws[0];
-      float x1 = xs[p.kblocks > 1 ? p.xs_bs : 0], w1 = ws[p.kblocks > 1 ? p.ws_bs : 0];
-      for (int kb = 0; kb < p.kblocks; ++kb, ac.next()) {
-        const float sc = x0 * w0;
-        x0 = x1;
-        w0 = w1;
-        const int nxt = min(kb + 2, p.kblocks - 1);
-        x1 = xs[nxt * p.xs_bs];
-        w1 = ws[nxt * p.ws_bs];
+      for (int kb = 0; kb < p.kblocks; ++kb, ac.next(), sl.next()) {
         const int a = ac.i;
         // the warp leaves together: the loads below need all of its lanes
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag, p.status,
-                                               kDevTimeoutSoftmax))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinScale + sl.i), sl.phase, abort_flag,
+                                               p.status, kDevTimeoutSoftmax) &&
+                                         mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag,
+                                                   p.status, kDevTimeoutSoftmax))) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const volatile float* sp = scale_s + sl.i * kScaleFloats;
+        const float sc = sp[r_in] * sp[128 + wg];
         const uint64_t sc2 = f2_pack(sc, sc);
+        uint32_t r[2][32];
+        tmem_ld32(t_lane + a * kBN, r[0]);
 #pragma unroll
         for (int c = 0; c < kCols; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(t_lane + a * kBN + c, r);
-          tmem_wait_ld(r);
-          if (c + 32 == kCols) {  // read out: the buffer may take the next product
+          uint32_t(&cur)[32] = r[(c / 32) & 1];
+          tmem_wait_ld(cur);
+          if (c + 32 < kCols) {
+            tmem_ld32(t_lane + a * kBN + c + 32, r[(c / 32 + 1) & 1]);
+          } else {  // read out: the buffer may take the next product
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -384,7 +482,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const uint64_t v = f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+            const uint64_t v = f2_fma(f2_pack(__uint_as_float(cur[j]), __uint_as_float(cur[j + 1])),
                                       sc2, f2_pack(acc[c + j], acc[c + j + 1]));
             f2_unpack(v, acc[c + j], acc[c + j + 1]);
           }
@@ -392,16 +490,25 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       }
       if (!ok) break;
       // ---- bias, activation, rounding, store
-      const int have = p.n - col;  // columns of this warpgroup that exist
-      if (p.bias != nullptr) {
+      if (p.bias != nullptr) {  // through shared memory: every lane needs every column's
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < kCols; ++j)
-          if (j < have) acc[j] += __ldg(p.bias + col + j);
+        for (int i = 0; i < kCols / 32; ++i) bias_s[lane + 32 * i] = bias[i];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kCols; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(bias_s + j);
+          acc[j] += b.x;
+          acc[j + 1] += b.y;
+          acc[j + 2] += b.z;
+          acc[j + 3] += b.w;
+        }
       }
       if (p.act == kActGeluTanh) {
 #pragma unroll
         for (int j = 0; j < kCols; j += 2) gelu_tanh2(acc[j], acc[j + 1]);
       }
+      float inv = 1.f;
       if constexpr (kOut == kOutE4m3) {
         float am = 0.f;
 #pragma unroll
@@ -419,63 +526,50 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           }
           am = fmaxf(am, mine[(wg ^ 1) * 128 + r_in]);
         }
-        float inv;
         const float s = block_scale(am, inv);
-        if (live && have > 0) {
-          if (col % kBlock == 0)
-            p.out_scale[row * p.os_rs + static_cast<long long>(col / kBlock) * p.os_bs] = s;
-          uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.out_stride + col;
-          if (p.vec_out && have >= kCols) {
+        if (live && have > 0 && col % kBlock == 0)
+          p.out_scale[row * p.os_rs + static_cast<long long>(col / kBlock) * p.os_bs] = s;
+      }
+      constexpr int kElem = kOut == kOutBf16 ? 2 : kOut == kOutFloat ? 4 : 1;
+      if (p.tma_out) {
+        // 32 rows x kWide bytes at a time, 16-byte pieces swizzled as the
+        // tensor map says, so that lanes (rows) hit different banks
+        constexpr int kWide = kCols * kElem < 128 ? kCols * kElem : 128;
+        constexpr int kWideCols = kWide / kElem;
+        const uint32_t buf = sbase + Dm::kStore + warp * 4096;
+        const uint32_t mine = buf + lane * kWide;
+        const uint32_t swz = kWide == 128 ? (lane & 7) : kWide == 64 ? ((lane >> 1) & 3) : 0;
 #pragma unroll
-            for (int j = 0; j < kCols; j += 32) {
-              uint32_t q[8];
+        for (int c = 0; c < kCols; c += kWideCols) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                q[i] = pack_e4m3x4(acc[j + 4 * i] * inv, acc[j + 4 * i + 1] * inv,
-                                   acc[j + 4 * i + 2] * inv, acc[j + 4 * i + 3] * inv);
-              st_global_v8(o + j, q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < kCols; ++j)
-              if (j < have) o[j] = static_cast<uint8_t>(pack_e4m3x4(acc[j] * inv, 0.f, 0.f, 0.f));
+          for (int i = 0; i < kWide / 16; ++i) {
+            uint32_t q[4];
+            lin_pack16<kOut>(acc + c + i * (16 / kElem), inv, q);
+            st_shared_v4(mine + ((i ^ swz) << 4), q[0], q[1], q[2], q[3]);
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && c < have && row < p.m) lin_store(&tm_o, buf, col + c, row);
         }
-      } else if constexpr (kOut == kOutBf16) {
-        if (live && have > 0) {
-          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + col;
-          if (p.vec_out && have >= kCols) {
+      } else if (live) {
 #pragma unroll
-            for (int j = 0; j < kCols; j += 16)
-              st_global_v8(o + j, pack_bf16x2(acc[j], acc[j + 1]), pack_bf16x2(acc[j + 2], acc[j + 3]),
-                           pack_bf16x2(acc[j + 4], acc[j + 5]), pack_bf16x2(acc[j + 6], acc[j + 7]),
-                           pack_bf16x2(acc[j + 8], acc[j + 9]), pack_bf16x2(acc[j + 10], acc[j + 11]),
-                           pack_bf16x2(acc[j + 12], acc[j + 13]),
-                           pack_bf16x2(acc[j + 14], acc[j + 15]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < kCols; ++j)
-              if (j < have) o[j] = __float2bfloat16(acc[j]);
-          }
-        }
-      } else {
-        if (live && have > 0) {
-          float* o = static_cast<float*>(p.out) + row * p.out_stride + col;
-          if (p.vec_out && have >= kCols) {
-#pragma unroll
-            for (int j = 0; j < kCols; j += 8)
-              st_global_v8(o + j, __float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
-                           __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]),
-                           __float_as_uint(acc[j + 4]), __float_as_uint(acc[j + 5]),
-                           __float_as_uint(acc[j + 6]), __float_as_uint(acc[j + 7]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < kCols; ++j)
-              if (j < have) o[j] = acc[j];
+        for (int j = 0; j < kCols; ++j) {
+          if (j < have) {
+            const long long at = row * p.out_stride + col + j;
+            if constexpr (kOut == kOutBf16)
+              static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(acc[j]);
+            else if constexpr (kOut == kOutFloat) static_cast<float*>(p.out)[at] = acc[j];
+            else
+              static_cast<uint8_t*>(p.out)[at] =
+                  static_cast<uint8_t>(pack_e4m3x4(acc[j] * inv, 0.f, 0.f, 0.f));
           }
         }
       }
     }
+    // the staged output has been read before the memory goes
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();

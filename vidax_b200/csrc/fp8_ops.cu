@@ -337,15 +337,24 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
     return fail(VX_EUNSUPPORTED, "too many output tiles (%lld)", tiles);
   p.tiles = static_cast<int>(tiles);
   p.act = a->activation;
-  p.vec_out = aligned(a->out, 32) && a->out_stride * type_size(a->out_type) % 32 == 0;
+  const int oe = type_size(a->out_type);
+  p.tma_out = aligned(a->out, 16) && a->out_stride * oe % 16 == 0;
   if ((rc = vx_internal_status_word(&p.status)) != VX_OK) return rc;
 
   // One row needs no stride; the map wants one that is a multiple of 16.
   const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
-  CUtensorMap tx, tw;
-  if ((rc = vx_internal_byte_tmap(&tx, a->x, a->k, a->m, xst, kLinRows)) != VX_OK) return rc;
-  if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, v.bn / v.cg)) != VX_OK) return rc;
+  CUtensorMap tx, tw, to;
+  if ((rc = vx_internal_byte_tmap(&tx, a->x, a->k, a->m, xst, 128, kLinRows)) != VX_OK) return rc;
+  if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, 128, v.bn / v.cg)) != VX_OK) return rc;
+  to = tx;  // not used without tma_out
+  if (p.tma_out) {
+    const uint64_t row = static_cast<uint64_t>(a->n) * oe;
+    const uint64_t ost = a->m > 1 ? static_cast<uint64_t>(a->out_stride) * oe : (row + 15) / 16 * 16;
+    if ((rc = vx_internal_byte_tmap(&to, a->out, row, a->m, ost, std::min(128, v.bn / 2 * oe), 32,
+                                    oe)) != VX_OK)
+      return rc;
+  }
   if ((rc = vx_internal_prepare_kernel(fn, dev, v.smem)) != VX_OK) return rc;
   int groups;
   if ((rc = resident_groups(v, fn, dev, sms, &groups)) != VX_OK) return rc;
@@ -361,7 +370,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  void* args[3] = {&tx, &tw, &p};
+  void* args[4] = {&tx, &tw, &to, &p};
   cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
   if (e != cudaSuccess) {
     cudaGetLastError();

@@ -185,18 +185,24 @@ int vx_internal_prepare_kernel(const void* fn, int dev, size_t smem) {
   return prepare_kernel(fn, dev, smem);
 }
 
-int vx_internal_byte_tmap(CUtensorMap* tm, const void* base, uint64_t cols, uint64_t rows,
-                          uint64_t stride, uint32_t box_rows) {
+int vx_internal_byte_tmap(CUtensorMap* tm, const void* base, uint64_t row_bytes, uint64_t rows,
+                          uint64_t stride, uint32_t box_bytes, uint32_t box_rows, int elem) {
   EncodeTiledFn enc;
   int rc = get_encode_fn(&enc);
   if (rc != VX_OK) return rc;
-  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t dims[2] = {row_bytes / elem, rows};
   const cuuint64_t strides[1] = {stride};
-  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t box[2] = {box_bytes / elem, box_rows};
   const cuuint32_t elem_str[2] = {1, 1};
-  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                   elem_str, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType type = elem == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUtensorMapSwizzle swizzle = box_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                       : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUresult r = enc(tm, type, 2, const_cast<void*>(base), dims, strides, box, elem_str,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(VX_EINVAL, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return VX_OK;
 }

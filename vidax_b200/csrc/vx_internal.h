@@ -23,8 +23,9 @@ int vx_internal_status_word(int** out);
 int vx_internal_device(int* dev, int* sms);
 int vx_internal_prepare_kernel(const void* fn, int dev, size_t smem);
 
-// 2-D tensor map over bytes: `rows` rows of `cols` bytes, `stride` bytes
-// apart, in boxes of 128 bytes x `box_rows`, 128-byte swizzled; reads past
-// the end give 0.
-int vx_internal_byte_tmap(CUtensorMap* tm, const void* base, uint64_t cols, uint64_t rows,
-                          uint64_t stride, uint32_t box_rows);
+// 2-D tensor map over `rows` rows of `row_bytes` bytes, `stride` bytes apart,
+// of elements of `elem` (1, 2 or 4) bytes, in boxes of box_bytes (128, 64 or
+// 32, swizzled over that width) x box_rows; loads read 0 past the end, stores
+// are clipped there.
+int vx_internal_byte_tmap(CUtensorMap* tm, const void* base, uint64_t row_bytes, uint64_t rows,
+                          uint64_t stride, uint32_t box_bytes, uint32_t box_rows, int elem = 1);
