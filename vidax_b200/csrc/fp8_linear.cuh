@@ -12,9 +12,9 @@
 // CTA roles (384 threads): warps 0-3 and 4-7 are two warpgroups that add up
 // the left and right half of the tile's columns (thread = row), warp 8 feeds
 // shared memory by TMA, warp 9 allocates TMEM and issues the MMAs, warp 10
-// fetches the scales (cp.async, any strides) as far ahead as warp 8 fetches
-// the operands: read from global memory where they are used, their latency
-// cost a third of the time of a long sum. CTAs are persistent: each strides
+// fetches the scales (cp.async, any strides) up to 16 blocks ahead: read from
+// global memory where they are used, their latency cost a third of the time
+// of a long sum. CTAs are persistent: each strides
 // over the output tiles, and the roles' barrier phases run on across tiles, so
 // the next tile's loads and products start while the last one is rounded and
 // stored. A finished tile leaves through shared memory by TMA (full 128-byte
@@ -55,7 +55,9 @@ struct LinearParams {
 constexpr int kLinThreads = 384;       // 3 warpgroups: two add and store, one feeds
 constexpr int kLinRows = 128;          // activation rows per CTA
 constexpr int kGroupM = 8;             // row tiles that share a pass over the weights
-constexpr int kScaleSlots = 16;        // blocks of scales in shared memory
+constexpr int kScaleGroups = 4;        // groups of scales in shared memory,
+constexpr int kGroupBlocks = 4;        // of this many blocks each
+constexpr int kScaleSlots = kScaleGroups * kGroupBlocks;
 constexpr int kScaleFloats = 132;      // 128 rows, 2 warpgroups' weight scales, padding
 // Registers: 384 threads start with 168 each; the feeding warpgroup gives 96
 // of its up and each adding one takes 48 (72 + 2 * 216 = 3 * 168), room for
@@ -72,9 +74,6 @@ struct LinDims {
   static constexpr int kFit = (232448 - 1024 - kRest) / kStageBytes;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kBufs = 512 / kBN < 4 ? 512 / kBN : 4;  // block products in TMEM
-  // A scale slot is written S blocks ahead of the tensor core, which is at
-  // most kBufs blocks ahead of the sums that read it.
-  static_assert(kStages + kBufs <= kScaleSlots, "scale slots");
   static constexpr uint32_t kStore = kStages * kStageBytes;
   static constexpr uint32_t kScales = kStore + kStoreBytes;
   static constexpr uint32_t kBias = kScales + kScaleSlots * kScaleFloats * 4;  // 128 floats per warp
@@ -92,8 +91,9 @@ enum : int {
   kLinAccEmpty = 20,   // 4: read by every adding warp (kCG = 2: both CTAs', at the leader)
   kLinAmax = 24,       // both warpgroups' largest magnitudes are written
   kLinDrain = 25,
-  kLinScale = 26,      // 16: a block's scales landed
-  kLinBars = 42,
+  kLinScaleFull = 26,  // 4: a group's scales landed
+  kLinScaleEmpty = 30, // 4: read by every adding warp
+  kLinBars = 34,
 };
 
 // Position in a ring of N barriers and the phase parity of its current round.
@@ -113,6 +113,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
+}
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok));
+  return ok != 0;
 }
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -290,7 +298,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   auto bar = [&](int i) -> uint32_t { return sbase + Dm::kCtl + 8u * i; };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Dm::kCtl + 8 * kLinBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Dm::kCtl + 8 * kLinBars + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The shuffle tells the compiler that the warp index is the same in all lanes.
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
   const uint32_t rank = kCG == 2 ? cluster_rank() : 0u;
   const int unit0 = blockIdx.x / kCG, unit_step = gridDim.x / kCG;
 
@@ -303,7 +313,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       mbar_init(bar(kLinAccFull + i), 1);
       mbar_init(bar(kLinAccEmpty + i), 8 * kCG);
     }
-    for (int i = 0; i < kScaleSlots; ++i) mbar_init(bar(kLinScale + i), 32);
+    for (int i = 0; i < kScaleGroups; ++i) {
+      mbar_init(bar(kLinScaleFull + i), 32);
+      mbar_init(bar(kLinScaleEmpty + i), 8);
+    }
     mbar_init(bar(kLinAmax), 256);
     mbar_init(bar(kLinDrain), 1);
     *abort_flag = 0;
@@ -318,82 +331,93 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   __syncthreads();
   if constexpr (kCG == 2) cluster_sync();  // the peer's barriers exist before anything arrives there
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFeedRegs));
   if (warp == 8) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      const uint64_t policy = l2_policy_evict_last();
-      Ring<S> st;
-      int filled = 0;  // stages that have been loaded at least once
-      bool ok = true;
-      for (int t = unit0; ok && t < p.tiles; t += unit_step) {
-        int tm, tn;
-        lin_tile(p, t, tm, tn);
-        const int row = (tm * kCG + rank) * kLinRows;
-        const int col = tn * kBN + rank * (kBN / kCG);
-        for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
-          const int s = st.i;
-          if (!mbar_wait(bar(kLinEmpty + s), st.phase ^ 1u, abort_flag, p.status,
-                         kDevTimeoutLoad)) {
-            ok = false;
-            break;
-          }
-          const uint32_t full = kCG == 2 ? map_to_rank(bar(kLinFull + s), 0) : bar(kLinFull + s);
-          if (rank == 0) mbar_expect_tx(bar(kLinFull + s), kCG * Dm::kStageBytes);
-          const uint32_t dst = sbase + s * Dm::kStageBytes;
+    const uint64_t policy = l2_policy_evict_last();
+    const bool issuer = elect_one();
+    const uint32_t full0 = kCG == 2 ? map_to_rank(bar(kLinFull), 0) : bar(kLinFull);
+    Ring<S> st;
+    int filled = 0;  // stages that have been loaded at least once
+    bool ok = true;
+    for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+      int tm, tn;
+      lin_tile(p, t, tm, tn);
+      const int row = (tm * kCG + rank) * kLinRows;
+      const int col = tn * kBN + rank * (kBN / kCG);
+      for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinEmpty + st.i), st.phase ^ 1u, abort_flag,
+                                               p.status, kDevTimeoutLoad))) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = full0 + 8u * st.i;
+        const uint32_t dst = sbase + st.i * Dm::kStageBytes;
+        if (issuer) {
+          if (rank == 0) mbar_expect_tx(bar(kLinFull + st.i), kCG * Dm::kStageBytes);
           lin_load<kCG>(dst, &tm_x, full, kb * kBlock, row, policy);
           lin_load<kCG>(dst + Dm::kABytes, &tm_w, full, kb * kBlock, col, policy);
-          if (filled < S) ++filled;
         }
+        __syncwarp();
+        if (filled < S) ++filled;
       }
-      if (!ok && rank == 0) {
-        // the loads in flight land before the CTA (pair) gives its memory back
-        for (int i = 0; i < filled; ++i) {
-          st.i = st.i == 0 ? S - 1 : st.i - 1;
-          if (st.i == S - 1) st.phase ^= 1u;
-          mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
-        }
+    }
+    if (!ok && rank == 0) {
+      // the loads in flight land before the CTA (pair) gives its memory back
+      for (int i = 0; i < filled; ++i) {
+        st.i = st.i == 0 ? S - 1 : st.i - 1;
+        if (st.i == S - 1) st.phase ^= 1u;
+        mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
       }
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one lane issues: addresses and
+    // descriptors then stay in uniform registers. With a single lane in the
+    // loop every MMA first moved its operands there, and the issuer (780
+    // cycles per block of a 256 x 256 tile) was slower than the tensor core (512).
+    if (rank == 0) {
       constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows * kCG, kBN);
+      const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
+      const bool issuer = elect_one();
       Ring<S> st;
       Ring<kBufs> ac;
       bool ok = true;
       for (int t = unit0; ok && t < p.tiles; t += unit_step) {
         for (int kb = 0; kb < p.kblocks; ++kb, st.next(), ac.next()) {
-          const int s = st.i, a = ac.i;
-          if (!mbar_wait(bar(kLinAccEmpty + a), ac.phase ^ 1u, abort_flag, p.status,
-                         kDevTimeoutMma) ||
-              !mbar_wait(bar(kLinFull + s), st.phase, abort_flag, p.status, kDevTimeoutMma)) {
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(bar(kLinAccEmpty + ac.i), ac.phase ^ 1u, abort_flag, p.status,
+                                    kDevTimeoutMma) &&
+                              mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status,
+                                        kDevTimeoutMma))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t base = sbase + s * Dm::kStageBytes;
-          const uint64_t da = sdesc_sw128(base, 16, 1024);
-          const uint64_t db = sdesc_sw128(base + Dm::kABytes, 16, 1024);
+          const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
+          const uint64_t db = da + (Dm::kABytes >> 4);
+          const uint32_t acc = tmem + ac.i * kBN;
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
-            lin_mma<kCG>(tmem + a * kBN, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
-          lin_commit<kCG>(bar(kLinEmpty + s));
-          lin_commit<kCG>(bar(kLinAccFull + a));
+            for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
+              lin_mma<kCG>(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
+            lin_commit<kCG>(bar(kLinEmpty + st.i));
+            lin_commit<kCG>(bar(kLinAccFull + ac.i));
+          }
+          __syncwarp();
         }
       }
-      if (!ok) {
+      if (!ok && issuer) {
         lin_commit<kCG>(bar(kLinDrain));
         mbar_wait_drain(bar(kLinDrain), 0, p.status);
       }
     }
   } else if (warp == 10) {
     // ------------------------------------------------------------ scales
-    Ring<S> st;
-    Ring<kScaleSlots> sl;
+    Ring<kScaleGroups> sg;
     bool ok = true;
     for (int t = unit0; ok && t < p.tiles; t += unit_step) {
       int tm, tn;
@@ -405,18 +429,21 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       for (int i = 0; i < 4; ++i)
         xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
       const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
-      for (int kb = 0; kb < p.kblocks; ++kb, st.next(), sl.next()) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinEmpty + st.i), st.phase ^ 1u, abort_flag,
+      for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag,
                                                p.status, kDevTimeoutLoad))) {
           ok = false;
           break;
         }
-        const uint32_t dst = sbase + Dm::kScales + sl.i * (kScaleFloats * 4) + lane * 4;
+        const int n = min(kGroupBlocks, p.kblocks - kb0);
+        uint32_t dst = sbase + Dm::kScales + sg.i * (kGroupBlocks * kScaleFloats * 4) + lane * 4;
+        for (int kb = kb0; kb < kb0 + n; ++kb, dst += kScaleFloats * 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
-        if (lane < 2) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
-        cp_async_arrive(bar(kLinScale + sl.i));
+          for (int i = 0; i < 4; ++i)
+            cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
+          if (lane < 2) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
+        }
+        cp_async_arrive(bar(kLinScaleFull + sg.i));
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -433,7 +460,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     float* amax_s = reinterpret_cast<float*>(smem + Dm::kAmax);
     const uint32_t empty0 = kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
     Ring<kBufs> ac;
-    Ring<kScaleSlots> sl;
+    Ring<kScaleGroups> sg;
     uint32_t tile_parity = 0;
     bool ok = true;
     for (int t = unit0; ok && t < p.tiles; t += unit_step, tile_parity ^= 1u) {
@@ -450,19 +477,25 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-      for (int kb = 0; kb < p.kblocks; ++kb, ac.next(), sl.next()) {
-        const int a = ac.i;
+      for (int kb = 0; kb < p.kblocks; ++kb, ac.next()) {
+        const int a = ac.i, in_group = kb % kGroupBlocks;
         // the warp leaves together: the loads below need all of its lanes
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinScale + sl.i), sl.phase, abort_flag,
-                                               p.status, kDevTimeoutSoftmax) &&
-                                         mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag,
-                                                   p.status, kDevTimeoutSoftmax))) {
+        if (!__all_sync(0xffffffffu,
+                        (in_group != 0 || mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag,
+                                                    p.status, kDevTimeoutSoftmax)) &&
+                            mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag, p.status,
+                                      kDevTimeoutSoftmax))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const volatile float* sp = scale_s + sl.i * kScaleFloats;
+        const volatile float* sp = scale_s + (sg.i * kGroupBlocks + in_group) * kScaleFloats;
         const float sc = sp[r_in] * sp[128 + wg];
+        if (in_group == kGroupBlocks - 1 || kb + 1 == p.kblocks) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
+          sg.next();
+        }
         const uint64_t sc2 = f2_pack(sc, sc);
         uint32_t r[2][32];
         tmem_ld32(t_lane + a * kBN, r[0]);
