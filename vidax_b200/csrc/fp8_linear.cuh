@@ -9,9 +9,9 @@
 // leaves TMEM and is added to a float32 sum in registers. The tensor core
 // works on the next blocks meanwhile: TMEM holds 512 / kBN block products.
 //
-// CTA roles (384 threads): warps 0-3 and 4-7 are two warpgroups that add up
-// the left and right half of the tile's columns (thread = row), warp 8 feeds
-// shared memory by TMA, warp 9 allocates TMEM and issues the MMAs, warp 10
+// CTA roles: two or four warpgroups each add up their share of the tile's
+// columns (thread = row); of the last warpgroup, the first warp feeds shared
+// memory by TMA, the second and the fourth issue the MMAs, the third
 // fetches the scales (cp.async, any strides) up to 16 blocks ahead: read from
 // global memory where they are used, their latency cost a third of the time
 // of a long sum. CTAs are persistent: each strides
@@ -52,33 +52,45 @@ struct LinearParams {
   int* status;
 };
 
-constexpr int kLinThreads = 384;       // 3 warpgroups: two add and store, one feeds
 constexpr int kLinRows = 128;          // activation rows per CTA
 constexpr int kGroupM = 8;             // row tiles that share a pass over the weights
 constexpr int kScaleGroups = 4;        // groups of scales in shared memory,
 constexpr int kGroupBlocks = 4;        // of this many blocks each
 constexpr int kScaleSlots = kScaleGroups * kGroupBlocks;
-constexpr int kScaleFloats = 132;      // 128 rows, 2 warpgroups' weight scales, padding
-// Registers: 384 threads start with 168 each; the feeding warpgroup gives 96
-// of its up and each adding one takes 48 (72 + 2 * 216 = 3 * 168), room for
-// 128 sums and a block product's next columns.
-constexpr int kFeedRegs = 72, kSumRegs = 216;
+constexpr int kScaleFloats = 132;      // 128 rows, the warpgroups' weight scales
 
 template <int kCG, int kBN>
 struct LinDims {
+  // Warpgroups that add: four for the widest tile (64 columns each), whose two
+  // block products in TMEM leave the reader the shortest time; four warps per
+  // SM quarter keep TMEM reads and additions going at once.
+  static constexpr int kSumWG = kBN == 256 ? 4 : 2;
+  static constexpr int kCols = kBN / kSumWG;
+  static constexpr int kThreads = 128 * (kSumWG + 1);
+  // Registers: the feeding warpgroup gives some of the launch's share up to
+  // the adding ones (640 threads: 96 each, 32 + 4 * 112 = 5 * 96; 384
+  // threads: 168 each, 56 + 2 * 224 = 3 * 168).
+  static constexpr int kFeedRegs = kSumWG == 4 ? 32 : 56;
+  static constexpr int kSumRegs = kSumWG == 4 ? 112 : 224;
   static constexpr uint32_t kABytes = kLinRows * kBlock;
   static constexpr uint32_t kBBytes = kBN / kCG * kBlock;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr uint32_t kStoreBytes = 8 * 4096;            // 32 rows x 128 bytes per warp
-  static constexpr uint32_t kRest = kStoreBytes + kScaleSlots * kScaleFloats * 4 + 8 * 512 + 2048 + 512;
+  static constexpr uint32_t kStoreBytes = kSumWG * 4 * 4096;   // 32 rows x 128 bytes per warp
+  static constexpr uint32_t kBiasBytes = kSumWG * 4 * kCols * 4;
+  static constexpr uint32_t kAmaxBytes = 2 * kSumWG * 512;     // 2 tiles x 128 rows
+  static constexpr uint32_t kRest =
+      kStoreBytes + kScaleSlots * kScaleFloats * 4 + kBiasBytes + kAmaxBytes + 512;
   static constexpr int kFit = (232448 - 1024 - kRest) / kStageBytes;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kBufs = 512 / kBN < 4 ? 512 / kBN : 4;  // block products in TMEM
+  // kLinDone serves the sums too: a stage comes round again only after they
+  // have read the products that came between.
+  static_assert(kStages > kBufs, "stages");
   static constexpr uint32_t kStore = kStages * kStageBytes;
   static constexpr uint32_t kScales = kStore + kStoreBytes;
-  static constexpr uint32_t kBias = kScales + kScaleSlots * kScaleFloats * 4;  // 128 floats per warp
-  static constexpr uint32_t kAmax = kBias + 8 * 512;           // 2 tiles x 256 floats
-  static constexpr uint32_t kCtl = kAmax + 2048;
+  static constexpr uint32_t kBias = kScales + kScaleSlots * kScaleFloats * 4;
+  static constexpr uint32_t kAmax = kBias + kBiasBytes;
+  static constexpr uint32_t kCtl = kAmax + kAmaxBytes;
   static constexpr uint32_t kSmemBytes = kCtl + 512 + 1024;    // + alignment
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
 };
@@ -86,14 +98,13 @@ struct LinDims {
 // control block: barriers, then the TMEM address and the abort flag
 enum : int {
   kLinFull = 0,        // stages: operands landed (kCG = 2: both CTAs', at the leader)
-  kLinEmpty = 8,       // stages: their MMAs are done
-  kLinAccFull = 16,    // 4: block product complete in TMEM
-  kLinAccEmpty = 20,   // 4: read by every adding warp (kCG = 2: both CTAs', at the leader)
-  kLinAmax = 24,       // both warpgroups' largest magnitudes are written
-  kLinDrain = 25,
-  kLinScaleFull = 26,  // 4: a group's scales landed
-  kLinScaleEmpty = 30, // 4: read by every adding warp
-  kLinBars = 34,
+  kLinDone = 8,        // stages: their MMAs are done (the stage is free, the product complete)
+  kLinAccEmpty = 16,   // 4: product read by every adding warp (kCG = 2: both CTAs', at the leader)
+  kLinAmax = 24,       // every warpgroup's largest magnitudes are written
+  kLinDrain = 26,      // 2: an issuer's MMAs are done (after an abort)
+  kLinScaleFull = 28,  // 4: a group's scales landed
+  kLinScaleEmpty = 32, // 4: read by every adding warp
+  kLinBars = 36,
 };
 
 // Position in a ring of N barriers and the phase parity of its current round.
@@ -285,12 +296,13 @@ __device__ __forceinline__ void lin_tile(const LinearParams& p, int t, int& tm, 
 }
 
 template <int kCG, int kBN, int kOut>
-__global__ void __launch_bounds__(kLinThreads, 1)
+__global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ LinearParams p) {
   using Dm = LinDims<kCG, kBN>;
   constexpr int S = Dm::kStages, kBufs = Dm::kBufs;
-  constexpr int kCols = kBN / 2;  // columns of a warpgroup
+  constexpr int kCols = Dm::kCols;  // columns of a warpgroup
+  constexpr int kFeed = 4 * Dm::kSumWG;  // first feeding warp
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -307,23 +319,21 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(bar(kLinFull + i), 1);
-      mbar_init(bar(kLinEmpty + i), 1);
+      mbar_init(bar(kLinDone + i), 1);
     }
-    for (int i = 0; i < kBufs; ++i) {
-      mbar_init(bar(kLinAccFull + i), 1);
-      mbar_init(bar(kLinAccEmpty + i), 8 * kCG);
-    }
+    for (int i = 0; i < kBufs; ++i) mbar_init(bar(kLinAccEmpty + i), kFeed * kCG);
     for (int i = 0; i < kScaleGroups; ++i) {
       mbar_init(bar(kLinScaleFull + i), 32);
-      mbar_init(bar(kLinScaleEmpty + i), 8);
+      mbar_init(bar(kLinScaleEmpty + i), kFeed);
     }
-    mbar_init(bar(kLinAmax), 256);
+    mbar_init(bar(kLinAmax), 32 * kFeed);
     mbar_init(bar(kLinDrain), 1);
+    mbar_init(bar(kLinDrain + 1), 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) lin_tmem_alloc<kCG>(sbase + Dm::kCtl + 8 * kLinBars);
-  if (warp == 8 && lane == 0) {
+  if (warp == kFeed + 1) lin_tmem_alloc<kCG>(sbase + Dm::kCtl + 8 * kLinBars);
+  if (warp == kFeed && lane == 0) {
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_w);
   }
@@ -333,9 +343,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFeedRegs));
-  if (warp == 8) {
+  if (warp >= kFeed) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Dm::kFeedRegs));
+  if (warp == kFeed) {
     // ------------------------------------------------------------ producer
     const uint64_t policy = l2_policy_evict_last();
     const bool issuer = elect_one();
@@ -349,7 +359,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       const int row = (tm * kCG + rank) * kLinRows;
       const int col = tn * kBN + rank * (kBN / kCG);
       for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinEmpty + st.i), st.phase ^ 1u, abort_flag,
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag,
                                                p.status, kDevTimeoutLoad))) {
           ok = false;
           break;
@@ -373,49 +383,58 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
       }
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer
-    // The whole warp walks the loop and one lane issues: addresses and
-    // descriptors then stay in uniform registers. With a single lane in the
-    // loop every MMA first moved its operands there, and the issuer (780
-    // cycles per block of a 256 x 256 tile) was slower than the tensor core (512).
+  } else if (warp == kFeed + 1 || warp == kFeed + 3) {
+    // ------------------------------------------------------------ MMA issuers
+    // Two warps take the blocks in turn: a block's two waits, four MMAs and
+    // commit take one issuer 500-600 cycles, a 256 x 256 x 128 product 512 and
+    // the smaller tiles' 256. Blocks are independent (each starts a product),
+    // so tiles do not matter here. The whole warp walks the loop and one lane
+    // issues: addresses and descriptors then stay in uniform registers.
     if (rank == 0) {
       constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows * kCG, kBN);
       const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
       const bool issuer = elect_one();
+      const int first = warp == kFeed + 3 ? 1 : 0;
+      const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
+      long long left = static_cast<long long>(tiles) * p.kblocks - first;
       Ring<S> st;
       Ring<kBufs> ac;
+      if (first) {
+        st.next();
+        ac.next();
+      }
       bool ok = true;
-      for (int t = unit0; ok && t < p.tiles; t += unit_step) {
-        for (int kb = 0; kb < p.kblocks; ++kb, st.next(), ac.next()) {
-          if (!__all_sync(0xffffffffu,
-                          mbar_wait(bar(kLinAccEmpty + ac.i), ac.phase ^ 1u, abort_flag, p.status,
-                                    kDevTimeoutMma) &&
-                              mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status,
-                                        kDevTimeoutMma))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
-          const uint64_t db = da + (Dm::kABytes >> 4);
-          const uint32_t acc = tmem + ac.i * kBN;
-          if (issuer) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
-              lin_mma<kCG>(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
-            lin_commit<kCG>(bar(kLinEmpty + st.i));
-            lin_commit<kCG>(bar(kLinAccFull + ac.i));
-          }
-          __syncwarp();
+      for (; left > 0; left -= 2) {
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status,
+                                  kDevTimeoutMma) &&
+                            mbar_wait(bar(kLinAccEmpty + ac.i), ac.phase ^ 1u, abort_flag, p.status,
+                                      kDevTimeoutMma))) {
+          ok = false;
+          break;
         }
+        tc_fence_after();
+        const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
+        const uint64_t db = da + (Dm::kABytes >> 4);
+        const uint32_t acc = tmem + ac.i * kBN;
+        if (issuer) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
+            lin_mma<kCG>(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
+          lin_commit<kCG>(bar(kLinDone + st.i));
+        }
+        __syncwarp();
+        st.next();
+        st.next();
+        ac.next();
+        ac.next();
       }
       if (!ok && issuer) {
-        lin_commit<kCG>(bar(kLinDrain));
-        mbar_wait_drain(bar(kLinDrain), 0, p.status);
+        lin_commit<kCG>(bar(kLinDrain + first));
+        mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == kFeed + 2) {
     // ------------------------------------------------------------ scales
     Ring<kScaleGroups> sg;
     bool ok = true;
@@ -423,7 +442,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       int tm, tn;
       lin_tile(p, t, tm, tn);
       const int row = (tm * kCG + rank) * kLinRows + lane;
-      const int col = tn * kBN + (lane & 1) * kCols;
+      const int col = tn * kBN + (lane & (Dm::kSumWG - 1)) * kCols;
       const float* xs[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -441,7 +460,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
-          if (lane < 2) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
+          if (lane < Dm::kSumWG) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
         }
         cp_async_arrive(bar(kLinScaleFull + sg.i));
       }
@@ -449,16 +468,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Dm::kSumRegs));
     // ------------------------------------------------------------ sums and output
     const int wg = warp >> 2;
     const int r_warp = (warp & 3) * 32;
     const int r_in = r_warp + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(r_warp) << 16) + wg * kCols;
     const float* scale_s = reinterpret_cast<const float*>(smem + Dm::kScales);
-    float* bias_s = reinterpret_cast<float*>(smem + Dm::kBias) + warp * 128;
+    float* bias_s = reinterpret_cast<float*>(smem + Dm::kBias) + warp * kCols;
     float* amax_s = reinterpret_cast<float*>(smem + Dm::kAmax);
     const uint32_t empty0 = kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
+    Ring<S> st;
     Ring<kBufs> ac;
     Ring<kScaleGroups> sg;
     uint32_t tile_parity = 0;
@@ -477,48 +497,46 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-      for (int kb = 0; kb < p.kblocks; ++kb, ac.next()) {
-        const int a = ac.i, in_group = kb % kGroupBlocks;
+      for (int kb = 0; kb < p.kblocks; ++kb, st.next(), ac.next()) {
+        const int in_group = kb % kGroupBlocks;
         // the warp leaves together: the loads below need all of its lanes
         if (!__all_sync(0xffffffffu,
                         (in_group != 0 || mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag,
                                                     p.status, kDevTimeoutSoftmax)) &&
-                            mbar_wait(bar(kLinAccFull + a), ac.phase, abort_flag, p.status,
+                            mbar_wait(bar(kLinDone + st.i), st.phase, abort_flag, p.status,
                                       kDevTimeoutSoftmax))) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const uint32_t tm_acc = t_lane + ac.i * kBN;
+        uint32_t r[32];
+        tmem_ld32(tm_acc, r);
         const volatile float* sp = scale_s + (sg.i * kGroupBlocks + in_group) * kScaleFloats;
         const float sc = sp[r_in] * sp[128 + wg];
-        if (in_group == kGroupBlocks - 1 || kb + 1 == p.kblocks) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
-          sg.next();
-        }
         const uint64_t sc2 = f2_pack(sc, sc);
-        uint32_t r[2][32];
-        tmem_ld32(t_lane + a * kBN, r[0]);
 #pragma unroll
         for (int c = 0; c < kCols; c += 32) {
-          uint32_t(&cur)[32] = r[(c / 32) & 1];
-          tmem_wait_ld(cur);
-          if (c + 32 < kCols) {
-            tmem_ld32(t_lane + a * kBN + c + 32, r[(c / 32 + 1) & 1]);
-          } else {  // read out: the buffer may take the next product
+          if (c > 0) tmem_ld32(tm_acc + c, r);
+          tmem_wait_ld(r);
+          if (c + 32 == kCols) {  // read out: the buffer may take the next product
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              if (kCG == 2) mbar_arrive_cluster(empty0 + 8u * a);
-              else mbar_arrive(empty0 + 8u * a);
+              if (kCG == 2) mbar_arrive_cluster(empty0 + 8u * ac.i);
+              else mbar_arrive(empty0 + 8u * ac.i);
             }
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const uint64_t v = f2_fma(f2_pack(__uint_as_float(cur[j]), __uint_as_float(cur[j + 1])),
-                                      sc2, f2_pack(acc[c + j], acc[c + j + 1]));
+            const uint64_t v = f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), sc2,
+                                      f2_pack(acc[c + j], acc[c + j + 1]));
             f2_unpack(v, acc[c + j], acc[c + j + 1]);
           }
+        }
+        if (in_group == kGroupBlocks - 1 || kb + 1 == p.kblocks) {
+          if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
+          sg.next();
         }
       }
       if (!ok) break;
@@ -546,10 +564,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         float am = 0.f;
 #pragma unroll
         for (int j = 0; j < kCols; ++j) am = fmaxf(am, fabsf(acc[j]));
-        if constexpr (kCols < kBlock) {  // the block's other columns are the other warpgroup's
+        if constexpr (kCols < kBlock) {  // the block's other columns are the next warpgroup's
           // Two copies by tile parity: a copy is written again only after the
           // next tile's barrier, which every reader of this one has passed.
-          volatile float* mine = amax_s + tile_parity * 256;
+          volatile float* mine = amax_s + tile_parity * (128 * Dm::kSumWG);
           mine[wg * 128 + r_in] = am;
           mbar_arrive(bar(kLinAmax));
           if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status,
@@ -610,7 +628,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   // both stay until both are done.
   if constexpr (kCG == 2) cluster_sync();
   tc_fence_after();
-  if (warp == 9) lin_tmem_dealloc<kCG>(tmem);
+  if (warp == kFeed + 1) lin_tmem_dealloc<kCG>(tmem);
 }
 
 }  // namespace fp8

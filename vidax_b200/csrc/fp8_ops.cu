@@ -92,6 +92,8 @@ struct LinVariant {
   int cg, bn;
   const void* fn[3];  // by output type
   uint32_t smem;
+  int threads;
+  int cols;           // columns of one warpgroup
 };
 
 template <int kCG, int kBN>
@@ -103,7 +105,9 @@ LinVariant variant() {
            kBN >= kBlock ? reinterpret_cast<const void*>(
                                &linear_kernel<kCG, (kBN >= kBlock ? kBN : kBlock), kOutE4m3>)
                          : nullptr},
-          LinDims<kCG, kBN>::kSmemBytes};
+          LinDims<kCG, kBN>::kSmemBytes,
+          LinDims<kCG, kBN>::kThreads,
+          LinDims<kCG, kBN>::kCols};
 }
 
 const LinVariant kVariants[] = {variant<2, 256>(), variant<2, 128>(), variant<1, 128>(),
@@ -124,7 +128,7 @@ int resident_groups(const LinVariant& v, const void* fn, int dev, int sms, int* 
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms / 2 * 2);
-    cfg.blockDim = dim3(kLinThreads);
+    cfg.blockDim = dim3(v.threads);
     cfg.dynamicSmemBytes = v.smem;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -351,7 +355,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   if (p.tma_out) {
     const uint64_t row = static_cast<uint64_t>(a->n) * oe;
     const uint64_t ost = a->m > 1 ? static_cast<uint64_t>(a->out_stride) * oe : (row + 15) / 16 * 16;
-    if ((rc = vx_internal_byte_tmap(&to, a->out, row, a->m, ost, std::min(128, v.bn / 2 * oe), 32,
+    if ((rc = vx_internal_byte_tmap(&to, a->out, row, a->m, ost, std::min(128, v.cols * oe), 32,
                                     oe)) != VX_OK)
       return rc;
   }
@@ -361,7 +365,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tiles, groups)) * v.cg);
-  cfg.blockDim = dim3(kLinThreads);
+  cfg.blockDim = dim3(v.threads);
   cfg.dynamicSmemBytes = v.smem;
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute at[1];
