@@ -47,7 +47,8 @@ def test_row_strides():
     assert _row_stride(t[..., ::2]) is None
     assert _row_stride(torch.zeros((1, 32)).expand(4, 32)) is None  # rows that lie on one another
     assert _row_stride(t[0, 0]) == 32
-    q = _empty_fp8((2, 5, 130), "cpu")
+    q, ld, ls = _empty_fp8((2, 5, 130), "cpu")
+    assert (ld, ls) == (144, 12)
     assert q.data.shape == (2, 5, 130) and _row_stride(q.data) == 144
     assert q.scale.shape == (2, 5, 2) and q.scale.flatten(0, 1).stride() == (1, 12)
 

@@ -5,19 +5,24 @@
 //   h = x + y * gate[batch]                 stored in the stream's type; the
 //                                           norm is that of the stored value
 //   m = 0 (RMS) or mean(h) (layer)
-//   n = (h - m) / sqrt(mean((h - m)^2) + eps) * w + b
-//   o = n * (1 + scale[batch]) + shift[batch]
+//   o = (h - m) / sqrt(mean((h - m)^2) + eps) * A + B
+//   A = w (1 + scale[batch]),  B = b (1 + scale[batch]) + shift[batch]
 //
 // HBM-bound: the row is read once and stays in registers between its
-// statistics and its output (W warps per row, NV vectors of eight features
-// per lane), so a float32 stream costs 4 + 2 bytes read and 4 + 1 written per
-// element. The separate gated addition and norm read it twice (16 bytes with
-// a bf16 output). The layer norm's variance is the mean of (h - m)^2 from
-// those registers, not E[h^2] - m^2, which loses digits when |m| is large.
-// A vector's features lie side by side in a lane, so a half-warp holds one
-// block of the e4m3 output and its largest magnitude is four shuffles away.
-// NV = 0 serves rows too wide for the registers: it reads the stored sum
-// again for each statistic and for the output.
+// statistics and its output (W warps per row, NV chunks of eight features per
+// lane), so a float32 stream costs 4 + 2 bytes read and 4 + 1 written per
+// element; a gated addition and a norm apart read it twice (16 bytes with a
+// bf16 output). The layer norm's variance is the mean of (h - m)^2 from those
+// registers, not E[h^2] - m^2, which loses digits when |m| is large.
+//
+// All of a row's loads are issued before anything is stored: a store between
+// them would order them (the stream may be updated in place), and the kernel
+// ran at 44 % of the measured copy bandwidth that way. For the same reason A,
+// B and the gate lie in shared memory, made once per CTA and batch item; a CTA
+// takes a run of neighbouring rows.
+//
+// add_norm_wide_kernel serves rows too wide for that (dim > 16384): it reads
+// the stored sum again for each statistic and for the output.
 #pragma once
 
 #include "fp8_common.cuh"
@@ -27,7 +32,7 @@ namespace fp8 {
 
 struct AddNormParams {
   const void* x;
-  void* sum;                  // NULL: the sum is not stored (no y)
+  void* sum;                  // with y
   const __nv_bfloat16* y;     // NULL: no addition
   const float* gate;          // (batches, dim) or NULL
   const float* w;             // (dim) or NULL
@@ -41,6 +46,7 @@ struct AddNormParams {
   long long out_scale_rs, out_scale_bs;
   long long rows;
   long long rows_per_batch;
+  long long rows_per_cta;
   int dim;
   int layer;                  // 1: LayerNorm, 0: RMSNorm
   float eps;
@@ -64,175 +70,220 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
   return v;
 }
 
-template <typename T>
-__device__ __forceinline__ float stored(float v);
-template <>
-__device__ __forceinline__ float stored<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float stored<__nv_bfloat16>(float v) {
+__device__ __forceinline__ float stored(float v, float) { return v; }
+__device__ __forceinline__ float stored(float v, __nv_bfloat16) {
   return __bfloat162float(__float2bfloat16(v));
 }
 
-// One row's addresses.
-template <typename T>
-struct AddNormRow {
-  const T* x;
-  T* sum;
-  const __nv_bfloat16* y;
-  const float *gate, *scale, *shift;
-  long long row;
-};
-
-// h of features [c, c + 8), of which `n` exist; stores the sum.
-template <typename T, bool kVec>
-__device__ __forceinline__ void add8(const AddNormParams& p, const AddNormRow<T>& r, int c, int n,
-                                     float (&h)[8]) {
-  load8<kVec>(r.x + (n > 0 ? c : 0), n, h);
-  if (p.y == nullptr) return;
-  float y[8];
-  load8<kVec>(r.y + (n > 0 ? c : 0), n, y);
-  if (r.gate != nullptr) {
-    float g[8];
-    load8<kVec>(r.gate + (n > 0 ? c : 0), n, g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = stored<T>(fmaf(y[i], g[i], h[i]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = stored<T>(h[i] + y[i]);
+// A and B of feature c of batch item bi.
+__device__ __forceinline__ void affine(const AddNormParams& p, long long bi, int c, float& a,
+                                       float& b) {
+  a = p.w != nullptr ? p.w[c] : 1.f;
+  b = p.b != nullptr ? p.b[c] : 0.f;
+  if (p.scale != nullptr) {
+    const float s = 1.f + p.scale[bi * p.scale_stride + c];
+    a *= s;
+    b *= s;
   }
-  if (n > 0) store8<kVec>(r.sum + c, n, h);
+  if (p.shift != nullptr) b += p.shift[bi * p.shift_stride + c];
 }
 
-// Normalises, modulates, rounds and stores features [c, c + 8).
-template <typename T, bool kVec>
-__device__ __forceinline__ void out8(const AddNormParams& p, const AddNormRow<T>& r, int c, int n,
-                                     float mean, float rstd, float (&h)[8]) {
-  const int cc = n > 0 ? c : 0;
-  float v[8];
+// The lane's eight values of a chunk of floats in shared memory.
+template <bool kVec>
+__device__ __forceinline__ void smem8(const float* chunk, int lane, float (&f)[8]) {
+  if constexpr (kVec) {
+    const float4 a = reinterpret_cast<const float4*>(chunk)[2 * lane];
+    const float4 b = reinterpret_cast<const float4*>(chunk)[2 * lane + 1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = (h[i] - mean) * rstd;
-  if (p.w != nullptr) {
-    load8<kVec>(p.w + cc, n, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] *= v[i];
+    for (int i = 0; i < 8; ++i) f[i] = chunk[i * 32 + lane];
   }
-  if (p.b != nullptr) {
-    load8<kVec>(p.b + cc, n, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] += v[i];
-  }
-  if (r.scale != nullptr) {
-    load8<kVec>(r.scale + cc, n, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] *= 1.f + v[i];
-  }
-  if (r.shift != nullptr) {
-    load8<kVec>(r.shift + cc, n, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] += v[i];
-  }
-  if (p.out_scale == nullptr) {
-    if (n > 0) store8<kVec>(static_cast<__nv_bfloat16*>(p.out) + r.row * p.out_stride + c, n, h);
-    return;
-  }
-  if (n < 8) {  // features past the row's end are not 0 any more
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i >= n) h[i] = 0.f;
-  }
-  float inv;
-  const float s = block_scale(half_warp_max(amax8(h)), inv);
-  if (n > 0) {
-    store8_e4m3<kVec>(static_cast<uint8_t*>(p.out) + r.row * p.out_stride + c, n, quantize8(h, inv));
-    if ((threadIdx.x & 15) == 0)
-      p.out_scale[r.row * p.out_scale_rs + static_cast<long long>(c / kBlock) * p.out_scale_bs] = s;
-  }
+}
+
+template <bool kVec>
+__device__ __forceinline__ void store_out(const AddNormParams& p, long long row, int c0, int lane,
+                                          int n, const float (&o)[8]) {
+  if (p.out_scale == nullptr)
+    store_chunk<kVec>(static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + c0, lane, n, o);
+  else
+    quantize_chunk<kVec>(static_cast<uint8_t*>(p.out) + row * p.out_stride + c0,
+                         p.out_scale + row * p.out_scale_rs + (c0 / kBlock) * p.out_scale_bs,
+                         p.out_scale_bs, lane, n, o);
 }
 
 template <typename T, int W, int NV, bool kVec>
 __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ AddNormParams p) {
   __shared__ float part[8];
-  const int lane_in_row = threadIdx.x & (32 * W - 1);
-  long long row = static_cast<long long>(blockIdx.x) * (8 / W) + (threadIdx.x / (32 * W));
-  // Rows past the end work on nothing but stay for the barriers and shuffles.
-  const int dim = row < p.rows ? p.dim : 0;
-  if (row >= p.rows) row = p.rows - 1;
-  const long long bi = row / p.rows_per_batch;
-  AddNormRow<T> r;
-  r.x = static_cast<const T*>(p.x) + row * p.x_stride;
-  r.sum = p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.sum_stride : nullptr;
-  r.y = p.y != nullptr ? p.y + row * p.y_stride : nullptr;
-  r.gate = p.gate != nullptr ? p.gate + bi * p.gate_stride : nullptr;
-  r.scale = p.scale != nullptr ? p.scale + bi * p.scale_stride : nullptr;
-  r.shift = p.shift != nullptr ? p.shift + bi * p.shift_stride : nullptr;
-  r.row = row;
+  extern __shared__ float4 norm_smem[];
+  constexpr int kCap = 256 * W * NV;  // features the CTA's registers hold
+  float* const sa = reinterpret_cast<float*>(norm_smem);
+  float* const sb = sa + kCap;
+  float* const sg = sb + kCap;  // with y only
+  const int lane = threadIdx.x & 31;
+  const int chunk0 = ((threadIdx.x >> 5) & (W - 1)) * 256;  // + 256 W v
   const float inv_n = 1.f / static_cast<float>(p.dim);
-  constexpr int kStep = 32 * W * 8;
-  if constexpr (NV > 0) {
-    float h[NV][8];
-    float s = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = v * kStep + lane_in_row * 8;
-      add8<T, kVec>(p, r, c, dim - c, h[v]);
-    }
-    float mean = 0.f;
-    if (p.layer) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += h[v][i];
-      mean = row_sum<W>(s, part) * inv_n;
-      s = 0.f;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int n = dim - (v * kStep + lane_in_row * 8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = i < n ? h[v][i] - mean : 0.f;
-        s = fmaf(d, d, s);
+  const long long last = min(p.rows, (blockIdx.x + 1LL) * p.rows_per_cta);
+  for (long long row0 = blockIdx.x * p.rows_per_cta; row0 < last;) {
+    const long long bi = row0 / p.rows_per_batch;
+    const long long end = min(last, (bi + 1) * p.rows_per_batch);
+    for (int c = threadIdx.x; c < kCap; c += 256) {  // past the row's end: 0
+      float a = 0.f, b = 0.f, g = 0.f;
+      if (c < p.dim) {
+        affine(p, bi, c, a, b);
+        g = p.gate != nullptr ? p.gate[bi * p.gate_stride + c] : 1.f;
       }
+      sa[c] = a;
+      sb[c] = b;
+      if (p.y != nullptr) sg[c] = g;
     }
-    const float rstd = 1.f / sqrtf(row_sum<W>(s, part) * inv_n + p.eps);
+    __syncthreads();
+    for (; row0 < end; row0 += 8 / W) {
+      // Rows past the segment's end work on its last row and store nothing,
+      // but stay for the barriers and shuffles.
+      const long long mine = row0 + threadIdx.x / (32 * W);
+      const bool live = mine < end;
+      const long long row = live ? mine : end - 1;
+      const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+      Raw<T, kVec> rx[NV];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = v * kStep + lane_in_row * 8;
-      out8<T, kVec>(p, r, c, dim - c, mean, rstd, h[v]);
-    }
-  } else {
-    float h[8];
-    float s = 0.f, s2 = 0.f;
-    for (int c0 = 0; c0 < p.dim; c0 += kStep) {
-      const int c = c0 + lane_in_row * 8;
-      add8<T, kVec>(p, r, c, dim - c, h);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s += h[i];
-        s2 = fmaf(h[i], h[i], s2);
+      for (int v = 0; v < NV; ++v) {
+        const int c0 = chunk0 + 256 * W * v;
+        rx[v].load(x + c0, lane, p.dim - c0);
       }
-    }
-    const T* src = p.y != nullptr ? r.sum : r.x;
-    float mean = 0.f;
-    if (p.layer) {
-      mean = row_sum<W>(s, part) * inv_n;
-      s2 = 0.f;
-      for (int c0 = 0; c0 < p.dim; c0 += kStep) {
-        const int c = c0 + lane_in_row * 8;
-        load8<kVec>(src + (dim > c ? c : 0), dim - c, h);
+      float h[NV][8];
+      if (p.y != nullptr) {
+        const __nv_bfloat16* y = p.y + row * p.y_stride;
+        Raw<__nv_bfloat16, kVec> ry[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c0 = chunk0 + 256 * W * v;
+          ry[v].load(y + c0, lane, p.dim - c0);
+        }
+        // In place is fine: each lane writes only the features it has read itself.
+        T* sum = static_cast<T*>(p.sum) + row * p.sum_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c0 = chunk0 + 256 * W * v;
+          float yv[8], g[8];
+          rx[v].get(h[v]);
+          ry[v].get(yv);
+          smem8<kVec>(sg + c0, lane, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[v][i] = stored(fmaf(yv[i], g[i], h[v][i]), T());
+          store_chunk<kVec>(sum + c0, lane, live ? p.dim - c0 : 0, h[v]);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) rx[v].get(h[v]);
+      }
+      float mean = 0.f, s = 0.f;
+      if (p.layer) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s += h[v][i];
+        mean = row_sum<W>(s, part) * inv_n;
+        s = 0.f;
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int n = p.dim - (chunk0 + 256 * W * v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float d = i < dim - c ? h[i] - mean : 0.f;
-          s2 = fmaf(d, d, s2);
+          h[v][i] -= mean;
+          const float d = feature<kVec>(lane, i) < n ? h[v][i] : 0.f;
+          s = fmaf(d, d, s);
         }
       }
+      const float rstd = 1.f / sqrtf(row_sum<W>(s, part) * inv_n + p.eps);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c0 = chunk0 + 256 * W * v;
+        float a[8], b[8];
+        smem8<kVec>(sa + c0, lane, a);
+        smem8<kVec>(sb + c0, lane, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[v][i] = fmaf(h[v][i] * rstd, a[i], b[i]);
+        store_out<kVec>(p, row, c0, lane, live ? p.dim - c0 : 0, h[v]);
+      }
     }
-    const float rstd = 1.f / sqrtf(row_sum<W>(s2, part) * inv_n + p.eps);
-    for (int c0 = 0; c0 < p.dim; c0 += kStep) {
-      const int c = c0 + lane_in_row * 8;
-      load8<kVec>(src + (dim > c ? c : 0), dim - c, h);
-      out8<T, kVec>(p, r, c, dim - c, mean, rstd, h);
+    row0 = end;
+    __syncthreads();  // A, B and the gate are read before the next batch item's are written
+  }
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constant__ AddNormParams p) {
+  __shared__ float part[8];
+  const int lane = threadIdx.x & 31;
+  const int chunk0 = (threadIdx.x >> 5) * 256;
+  const long long row = blockIdx.x;
+  const long long bi = row / p.rows_per_batch;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const float inv_n = 1.f / static_cast<float>(p.dim);
+  float s = 0.f, s2 = 0.f, mean = 0.f;
+  for (int c0 = chunk0; c0 < p.dim; c0 += 2048) {
+    const int n = p.dim - c0;
+    Raw<T, kVec> rx;
+    float h[8];
+    rx.load(x + c0, lane, n);
+    rx.get(h);
+    if (p.y != nullptr) {
+      Raw<__nv_bfloat16, kVec> ry;
+      Raw<float, kVec> rg;
+      float y[8], g[8];
+      ry.load(p.y + row * p.y_stride + c0, lane, n);
+      ry.get(y);
+      if (p.gate != nullptr) {
+        rg.load(p.gate + bi * p.gate_stride + c0, lane, n);
+        rg.get(g);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        h[i] = stored(p.gate != nullptr ? fmaf(y[i], g[i], h[i]) : h[i] + y[i], T());
+      store_chunk<kVec>(static_cast<T*>(p.sum) + row * p.sum_stride + c0, lane, n, h);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s += h[i];
+      s2 = fmaf(h[i], h[i], s2);
+    }
+  }
+  // each lane reads again what it wrote itself
+  const T* src = p.y != nullptr ? static_cast<const T*>(p.sum) + row * p.sum_stride : x;
+  if (p.layer) {
+    mean = row_sum<8>(s, part) * inv_n;
+    s2 = 0.f;
+    for (int c0 = chunk0; c0 < p.dim; c0 += 2048) {
+      const int n = p.dim - c0;
+      Raw<T, kVec> rx;
+      float h[8];
+      rx.load(src + c0, lane, n);
+      rx.get(h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = feature<kVec>(lane, i) < n ? h[i] - mean : 0.f;
+        s2 = fmaf(d, d, s2);
+      }
+    }
+  }
+  const float rstd = 1.f / sqrtf(row_sum<8>(s2, part) * inv_n + p.eps);
+  for (int c0 = chunk0; c0 < p.dim; c0 += 2048) {
+    const int n = p.dim - c0;
+    Raw<T, kVec> rx;
+    float h[8];
+    rx.load(src + c0, lane, n);
+    rx.get(h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = feature<kVec>(lane, i);
+      float a = 0.f, b = 0.f;
+      if (c < n) affine(p, bi, c0 + c, a, b);
+      h[i] = fmaf((h[i] - mean) * rstd, a, b);
+    }
+    store_out<kVec>(p, row, c0, lane, n, h);
   }
 }
 

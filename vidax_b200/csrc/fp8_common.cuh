@@ -35,89 +35,151 @@ __device__ __forceinline__ float block_scale(float amax, float& inv) {
   return a * (1.f / kMax);
 }
 
-__device__ __forceinline__ float amax8(const float (&f)[8]) {
-  float m = fmaxf(fabsf(f[0]), fabsf(f[1]));
-#pragma unroll
-  for (int i = 2; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
-  return m;
-}
-
-// Largest value over each half-warp (16 lanes x 8 elements = one block of a row).
-__device__ __forceinline__ float half_warp_max(float m) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float inv) {
-  return make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                    pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-}
-
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight consecutive elements at `p`, of which the first `n` exist (0 for the
-// rest). kVec: `p` is 16-byte aligned (8 bf16) / 32-byte aligned (8 float).
+__device__ __forceinline__ float amax4(float a, float b, float c, float d) {
+  return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d)));
+}
+template <int kLanes>
+__device__ __forceinline__ float lanes_max(float m) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// A warp's 256 consecutive features of a row, eight per lane. kVec (rows of
+// 8 k features on 16-byte boundaries): lane l holds features 8 l .. 8 l + 7,
+// moved as vectors; a half-warp then holds one block of 128. Otherwise lane l
+// holds features l, l + 32, ..., so that a warp's element accesses are
+// neighbours; elements 0-3 and 4-7 of all lanes are the two blocks.
 template <bool kVec>
-__device__ __forceinline__ void load8(const float* p, int n, float (&f)[8]) {
-  if (kVec && n >= 8) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0];
-    const float4 b = reinterpret_cast<const float4*>(p)[1];
+__device__ __forceinline__ int feature(int lane, int i) {
+  return kVec ? lane * 8 + i : i * 32 + lane;
+}
+
+// The lane's eight elements as they lie in memory (`row` points at the chunk,
+// of which the first `n` features exist; the others read 0).
+template <typename T, bool kVec>
+struct Raw;
+template <>
+struct Raw<float, true> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* row, int lane, int n) {
+    a = b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane * 8 < n) {
+      a = reinterpret_cast<const float4*>(row)[2 * lane];
+      b = reinterpret_cast<const float4*>(row)[2 * lane + 1];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : 0.f;
   }
-}
-template <bool kVec>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, float (&f)[8]) {
-  if (kVec && n >= 8) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
+};
+template <>
+struct Raw<__nv_bfloat16, true> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane, int n) {
+    a = make_uint4(0u, 0u, 0u, 0u);
+    if (lane * 8 < n) a = reinterpret_cast<const uint4*>(row)[lane];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       f[2 * k] = __uint_as_float(w[k] << 16);
       f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
     }
+  }
+};
+template <>
+struct Raw<float, false> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* row, int lane, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = 0.f;
+      if (i * 32 + lane < n) v[i] = row[i * 32 + lane];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = v[i];
+  }
+};
+template <>
+struct Raw<__nv_bfloat16, false> {
+  uint16_t v[8];
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane, int n) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = 0;
+      if (i * 32 + lane < n) v[i] = p[i * 32 + lane];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(static_cast<uint32_t>(v[i]) << 16);
+  }
+};
+
+template <bool kVec>
+__device__ __forceinline__ void store_chunk(float* row, int lane, int n, const float (&f)[8]) {
+  if constexpr (kVec) {
+    if (lane * 8 < n) {
+      reinterpret_cast<float4*>(row)[2 * lane] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(row)[2 * lane + 1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < n) row[i * 32 + lane] = f[i];
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store_chunk(__nv_bfloat16* row, int lane, int n, const float (&f)[8]) {
+  if constexpr (kVec) {
+    if (lane * 8 < n)
+      reinterpret_cast<uint4*>(row)[lane] =
+          make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                     pack_bf16x2(f[6], f[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < n) row[i * 32 + lane] = __float2bfloat16(f[i]);
   }
 }
 
+// Quantises and stores the chunk (features past the end must be 0); `scale`
+// points at the scale of its first block, the second is `bs` floats on.
 template <bool kVec>
-__device__ __forceinline__ void store8(float* p, int n, const float (&f)[8]) {
-  if (kVec && n >= 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void quantize_chunk(uint8_t* row, float* scale, long long bs, int lane,
+                                               int n, const float (&f)[8]) {
+  const float lo = amax4(f[0], f[1], f[2], f[3]), hi = amax4(f[4], f[5], f[6], f[7]);
+  float inv;
+  if constexpr (kVec) {
+    const float s = block_scale(lanes_max<16>(fmaxf(lo, hi)), inv);
+    if (lane * 8 < n) {
+      reinterpret_cast<uint2*>(row)[lane] =
+          make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                     pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+      if ((lane & 15) == 0) scale[(lane >> 4) * bs] = s;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = f[i];
-  }
-}
-template <bool kVec>
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const float (&f)[8]) {
-  if (kVec && n >= 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                              pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else {
+    for (int half = 0; half < 2; ++half) {
+      const float s = block_scale(lanes_max<32>(half ? hi : lo), inv);
+      const uint32_t q = pack_e4m3x4(f[4 * half] * inv, f[4 * half + 1] * inv,
+                                     f[4 * half + 2] * inv, f[4 * half + 3] * inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = __float2bfloat16(f[i]);
-  }
-}
-// Eight e4m3 bytes; kVec: `p` 8-byte aligned.
-template <bool kVec>
-__device__ __forceinline__ void store8_e4m3(uint8_t* p, int n, uint2 q) {
-  if (kVec && n >= 8) {
-    *reinterpret_cast<uint2*>(p) = q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+      for (int i = 0; i < 4; ++i) {
+        const int c = (4 * half + i) * 32 + lane;
+        if (c < n) row[c] = static_cast<uint8_t>(q >> (8 * i));
+      }
+      if (lane == 0 && half * kBlock < n) scale[half * bs] = s;
+    }
   }
 }
 

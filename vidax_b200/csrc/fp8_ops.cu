@@ -52,7 +52,7 @@ int check_scale(const char* name, const void* p, const int64_t (&st)[2]) {
   return VX_OK;
 }
 
-// A vector of 8 elements starts at each multiple of 8 of every row.
+// Rows of 8 k elements on 16-byte boundaries (8-byte ones of 1-byte elements).
 bool vec8(const void* p, int64_t stride, int elem) {
   const int64_t bytes = std::min(8 * elem, 16);
   return aligned(p, bytes) && stride * elem % bytes == 0;
@@ -60,30 +60,60 @@ bool vec8(const void* p, int64_t stride, int elem) {
 
 // ------------------------------------------------------------------ add_norm
 
-template <typename T, bool kVec>
-void launch_add_norm(const AddNormParams& p, int sms, cudaStream_t s) {
-  // Warps per row: one while its vectors fit a lane's registers, more for
-  // wide rows, and more where there are too few rows to fill the GPU with one
-  // warp each (a row's latency then counts, not its bandwidth).
-  const int vecs = (p.dim + 7) / 8;
-  auto go = [&](auto kernel, int w) {
-    const long long per = 8 / w;
-    kernel<<<static_cast<unsigned>((p.rows + per - 1) / per), 256, 0, s>>>(p);
-  };
-  const bool few = p.rows < 4LL * sms;
-  if (vecs <= 32) return go(add_norm_kernel<T, 1, 1, kVec>, 1);
-  if (!few) {
-    if (vecs <= 64) return go(add_norm_kernel<T, 1, 2, kVec>, 1);
-    if (vecs <= 128) return go(add_norm_kernel<T, 1, 4, kVec>, 1);
-    if (vecs <= 192) return go(add_norm_kernel<T, 1, 6, kVec>, 1);
+std::mutex g_norm_mu;
+std::map<std::pair<const void*, int>, int> g_norm_ctas;
+
+template <typename T, int W, int NV, bool kVec>
+int launch_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
+  const void* fn = reinterpret_cast<const void*>(&add_norm_kernel<T, W, NV, kVec>);
+  constexpr size_t kFull = 3u * 256 * W * NV * sizeof(float);
+  const size_t smem = p.y != nullptr ? kFull : kFull / 3 * 2;
+  int rc = vx_internal_prepare_kernel(fn, dev, kFull);
+  if (rc != VX_OK) return rc;
+  int per_sm;
+  {
+    std::lock_guard<std::mutex> lk(g_norm_mu);
+    int& n = g_norm_ctas[{fn, dev}];
+    if (n == 0) {
+      cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 256, kFull);
+      if (e != cudaSuccess) return vx_internal_cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+      n = std::max(n, 1);
+    }
+    per_sm = n;
   }
-  if (vecs <= 128) return go(add_norm_kernel<T, 4, 1, kVec>, 4);
-  if (vecs <= 256) return go(add_norm_kernel<T, 4, 2, kVec>, 4);
-  if (vecs <= 512) return go(add_norm_kernel<T, 4, 4, kVec>, 4);
-  if (vecs <= 640) return go(add_norm_kernel<T, 4, 5, kVec>, 4);
-  if (vecs <= 1024) return go(add_norm_kernel<T, 8, 4, kVec>, 8);
-  if (vecs <= 2048) return go(add_norm_kernel<T, 8, 8, kVec>, 8);
-  return go(add_norm_kernel<T, 8, 0, kVec>, 8);
+  constexpr int kPer = 8 / W;  // rows at a time
+  const long long groups = (p.rows + kPer - 1) / kPer;
+  const long long ctas = std::min<long long>(groups, static_cast<long long>(sms) * per_sm);
+  p.rows_per_cta = (groups + ctas - 1) / ctas * kPer;
+  const long long grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
+  add_norm_kernel<T, W, NV, kVec><<<static_cast<unsigned>(grid), 256, smem, s>>>(p);
+  return VX_OK;
+}
+
+template <typename T, bool kVec>
+int launch_add_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
+  // Warps per row: one while the row fits a lane's registers, more for wide
+  // rows, and more where there are too few rows to fill the GPU with one warp
+  // each (a row's latency then counts, not its bandwidth).
+  const int vecs = (p.dim + 255) / 256;
+  const bool few = p.rows < 4LL * sms;
+  if (vecs <= 1) return launch_norm<T, 1, 1, kVec>(p, dev, sms, s);
+  if (!few) {
+    if (vecs <= 2) return launch_norm<T, 1, 2, kVec>(p, dev, sms, s);
+    if (vecs <= 4) return launch_norm<T, 1, 4, kVec>(p, dev, sms, s);
+    if (vecs <= 6) return launch_norm<T, 1, 6, kVec>(p, dev, sms, s);
+  }
+  if (vecs <= 4) return launch_norm<T, 4, 1, kVec>(p, dev, sms, s);
+  if (vecs <= 8) return launch_norm<T, 4, 2, kVec>(p, dev, sms, s);
+  if (vecs <= 12) return launch_norm<T, 4, 3, kVec>(p, dev, sms, s);
+  if (vecs <= 16) return launch_norm<T, 4, 4, kVec>(p, dev, sms, s);
+  if (vecs <= 20) return launch_norm<T, 4, 5, kVec>(p, dev, sms, s);
+  if (vecs <= 32) return launch_norm<T, 8, 4, kVec>(p, dev, sms, s);
+  if (vecs <= 40) return launch_norm<T, 8, 5, kVec>(p, dev, sms, s);
+  if (vecs <= 56) return launch_norm<T, 8, 7, kVec>(p, dev, sms, s);
+  if (vecs <= 64) return launch_norm<T, 8, 8, kVec>(p, dev, sms, s);
+  add_norm_wide_kernel<T, kVec><<<static_cast<unsigned>(p.rows), 256, 0, s>>>(p);
+  return VX_OK;
 }
 
 // ------------------------------------------------------------------ linear
@@ -187,24 +217,24 @@ extern "C" int vx_quantize_fp8(const vx_quantize_fp8_args* a, vx_stream_t stream
   p.scale_bs = a->scale_stride[1];
   p.rows = a->rows;
   p.dim = a->dim;
-  p.blocks = (a->dim - 1) / kBlock + 1;
-  const int per = a->block_rows == 1 ? kRows : kBlock;
-  const long long items = (a->rows + per - 1) / per * p.blocks;
-  if (items > INT_MAX) return fail(VX_EUNSUPPORTED, "too many blocks (%lld)", items);
+  const bool by_row = a->block_rows == 1;
+  const int per = by_row ? kRows : kBlock;
+  p.chunks = (a->dim - 1) / (by_row ? 2 * kBlock : kBlock) + 1;
+  const long long items = ((a->rows - 1) / per + 1) * p.chunks;
+  if (a->rows > INT_MAX || items > INT_MAX) return fail(VX_EUNSUPPORTED, "too many blocks");
   p.items = static_cast<unsigned>(items);
-  p.vec_scale = p.scale_rs == 1 && p.scale_bs % kRows == 0 && aligned(p.scale, 16);
-  const bool vec = vec8(p.src, p.src_stride, elem) && vec8(p.dst, p.dst_stride, 1);
+  const bool vec =
+      a->dim % 8 == 0 && vec8(p.src, p.src_stride, elem) && vec8(p.dst, p.dst_stride, 1);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto rows_kernel, auto tiles_kernel) {
-    if (a->block_rows == 1) rows_kernel<<<(p.items + 15) / 16, 256, 0, s>>>(p);
-    else tiles_kernel<<<p.items, 256, 0, s>>>(p);
-  };
+  const unsigned grid = by_row ? (p.items + 7) / 8 : p.items;
   if (a->src_type == VX_TYPE_FLOAT) {
-    if (vec) go(quantize_rows_kernel<float, true>, quantize_tiles_kernel<float, true>);
-    else go(quantize_rows_kernel<float, false>, quantize_tiles_kernel<float, false>);
+    if (!by_row) quantize_tiles_kernel<float><<<grid, 256, 0, s>>>(p);
+    else if (vec) quantize_rows_kernel<float, true><<<grid, 256, 0, s>>>(p);
+    else quantize_rows_kernel<float, false><<<grid, 256, 0, s>>>(p);
   } else {
-    if (vec) go(quantize_rows_kernel<__nv_bfloat16, true>, quantize_tiles_kernel<__nv_bfloat16, true>);
-    else go(quantize_rows_kernel<__nv_bfloat16, false>, quantize_tiles_kernel<__nv_bfloat16, false>);
+    if (!by_row) quantize_tiles_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+    else if (vec) quantize_rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, s>>>(p);
+    else quantize_rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, s>>>(p);
   }
   return launched("quantize_fp8 launch");
 }
@@ -228,7 +258,7 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
   int rc;
   if ((rc = check_rows("x", a->x, a->x_stride, a->rows, a->dim, xe)) != VX_OK) return rc;
   if ((rc = check_rows("out", a->out, a->out_stride, a->rows, a->dim, oe)) != VX_OK) return rc;
-  bool vec = vec8(a->x, a->x_stride, xe) && vec8(a->out, a->out_stride, oe);
+  bool vec = a->dim % 8 == 0 && vec8(a->x, a->x_stride, xe) && vec8(a->out, a->out_stride, oe);
   if (a->y != nullptr) {
     if ((rc = check_rows("y", a->y, a->y_stride, a->rows, a->dim, 2)) != VX_OK) return rc;
     if ((rc = check_rows("sum", a->sum, a->sum_stride, a->rows, a->dim, xe)) != VX_OK) return rc;
@@ -241,7 +271,7 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
     if (vs[i] == nullptr) continue;
     if (!aligned(vs[i], 4)) return fail(VX_EINVAL, "%s is not aligned to its element", names[i]);
     if (vst[i] < 0) return fail(VX_EINVAL, "%s has a negative stride", names[i]);
-    vec = vec && vec8(vs[i], vst[i], 4);
+    if (a->dim > 16384) vec = vec && vec8(vs[i], vst[i], 4);  // the others go through shared memory
   }
   if (a->out_type == VX_TYPE_E4M3 &&
       (rc = check_scale("out_scale", a->out_scale, a->out_scale_stride)) != VX_OK)
@@ -275,13 +305,12 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
   p.layer = a->norm == VX_NORM_LAYER;
   p.eps = a->eps;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->x_type == VX_TYPE_FLOAT) {
-    if (vec) launch_add_norm<float, true>(p, sms, s);
-    else launch_add_norm<float, false>(p, sms, s);
-  } else {
-    if (vec) launch_add_norm<__nv_bfloat16, true>(p, sms, s);
-    else launch_add_norm<__nv_bfloat16, false>(p, sms, s);
-  }
+  if (a->x_type == VX_TYPE_FLOAT)
+    rc = vec ? launch_add_norm<float, true>(p, dev, sms, s) : launch_add_norm<float, false>(p, dev, sms, s);
+  else
+    rc = vec ? launch_add_norm<__nv_bfloat16, true>(p, dev, sms, s)
+             : launch_add_norm<__nv_bfloat16, false>(p, dev, sms, s);
+  if (rc != VX_OK) return rc;
   return launched("add_norm launch");
 }
 

@@ -18,6 +18,7 @@ Inference only, like the rest of this package: the outputs carry no gradient.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -91,18 +92,37 @@ class Fp8Tensor(NamedTuple):
         return self.data.float() * s
 
 
+_entries = {}
+
+
 def _entry(name: str, args):
-    fn = getattr(_lib.load(), name)
-    fn.argtypes = [ctypes.POINTER(type(args)), ctypes.c_void_p]
-    fn.restype = ctypes.c_int
+    """The C entry point `name`, its argument types set once."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(_lib.load(), name)
+        fn.argtypes = [ctypes.POINTER(type(args)), ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+        _entries[name] = fn
     return fn
 
 
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# torch's own lookup of the handle, without the Stream object around it (3 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 def _launch(name: str, args, device: torch.device) -> None:
-    fn = _entry(name, args)
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device)
-        _lib.check(fn(ctypes.byref(args), ctypes.c_void_p(stream.cuda_stream)))
+    fn = _entries.get(name) or _entry(name, args)
+    if device.index == torch.cuda.current_device():
+        rc = fn(args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(args, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc)
 
 
 def _check_cuda(name: str, t, dtypes, min_dim: int = 1) -> None:
@@ -122,14 +142,17 @@ def _check_cuda(name: str, t, dtypes, min_dim: int = 1) -> None:
 def _row_stride(t: torch.Tensor) -> Optional[int]:
     """Elements between the consecutive rows (..., K) -> (rows, K) of `t`
     without a copy, or None where they are not evenly spaced."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    k = t.shape[-1]
+    if t.is_contiguous():
+        return k
+    if k > 1 and t.stride(-1) != 1:
         return None
     dims = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
     for (_, s0), (n1, s1) in zip(dims, dims[1:]):
         if s0 != n1 * s1:
             return None
-    stride = dims[-1][1] if dims else t.shape[-1]
-    return stride if stride >= t.shape[-1] else None
+    stride = dims[-1][1] if dims else k
+    return stride if stride >= k else None
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -141,21 +164,22 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, s
 
 
-def _empty_fp8(shape, device) -> Fp8Tensor:
+def _empty_fp8(shape, device) -> Tuple[Fp8Tensor, int, int]:
     """An activation's storage: rows on 16-byte boundaries (the matrix
     product's loads need that), the scales of one block of features side by
-    side (a warp of the matrix product reads those of 32 rows at once)."""
+    side (a warp of the matrix product reads those of 32 rows at once, the
+    quantiser writes those of four). Returns it with the elements between its
+    rows and between its blocks of scales."""
     *lead, k = shape
-    rows = 1
-    for n in lead:
-        rows *= n
-    ld = -(-k // 16) * 16
-    data = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)[:, :k]
-    ls = -(-rows // 4) * 4
-    scale = torch.empty((-(-k // BLOCK), ls), dtype=torch.float32, device=device)[:, :rows].t()
-    if len(lead) == 1:
-        return Fp8Tensor(data, scale)
-    return Fp8Tensor(data.unflatten(0, lead), scale.unflatten(0, lead))
+    rows = math.prod(lead)
+    ld, ls = -(-k // 16) * 16, -(-rows // 4) * 4
+    sd, ss = [ld, 1], [1, ls]
+    for n in reversed(lead[1:]):
+        sd.insert(0, sd[0] * n)
+        ss.insert(0, ss[0] * n)
+    data = torch.empty_strided(shape, sd, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty_strided((*lead, -(-k // BLOCK)), ss, dtype=torch.float32, device=device)
+    return Fp8Tensor(data, scale), ld, ls
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
@@ -175,40 +199,43 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
         raise ValueError(f"a weight is (N, K), got {tuple(x.shape)}")
     if x.shape[-1] < 1:
         raise ValueError("x has no features")
-    out = _empty_fp8(x.shape, x.device)
+    dev = x.device
+    rows, k = math.prod(x.shape[:-1]), x.shape[-1]
+    out, ld, ls = _empty_fp8(x.shape, dev)
+    rs = 1
     if block_rows == BLOCK:
-        out = Fp8Tensor(out.data, torch.empty((-(-x.shape[0] // BLOCK), out.scale.shape[-1]),
-                                              dtype=torch.float32, device=x.device))
-    if x.numel() == 0:
+        rs, ls = -(-k // BLOCK), 1
+        out = Fp8Tensor(out.data, torch.empty((-(-rows // BLOCK), rs), dtype=torch.float32, device=dev))
+    if rows == 0:
         return out
     x, stride = _rows(x)
-    a = QuantizeFp8Args()
-    a.src, a.dst, a.scale = x.data_ptr(), out.data.data_ptr(), out.scale.data_ptr()
-    a.src_stride, a.dst_stride = stride, _row_stride(out.data)
-    a.scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
-    a.rows, a.dim = x.numel() // x.shape[-1], x.shape[-1]
-    a.src_type, a.block_rows = _TYPES[x.dtype], block_rows
-    _launch("vx_quantize_fp8", a, x.device)
+    _launch("vx_quantize_fp8", QuantizeFp8Args(
+        x.data_ptr(), out.data.data_ptr(), out.scale.data_ptr(), stride, ld, (rs, ls), rows, k,
+        _TYPES[x.dtype], block_rows), dev)
     return out
 
 
 def _vector(name: str, t: Optional[torch.Tensor], shape, device):
     """A float32 vector (dim) or per-batch-item vector (B, dim) / (B, 1, dim)
-    in place (converted where its type or layout differs)."""
+    in place (converted where its type or layout differs): its address, its
+    stride between batch items, and the tensor that holds it."""
     if t is None:
-        return None, 0
+        return None, 0, None
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} requires a gradient: this operator is inference only")
     if t.device != device:
         raise ValueError(f"{name} must live on x's device")
     if t.dim() == 3 and len(shape) == 2 and t.shape[1] == 1:
         t = t[:, 0]
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    t = t.detach().to(torch.float32)
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         t = t.contiguous()
-    return t, (t.stride(0) if len(shape) == 2 and shape[0] > 1 else 0)
+    return t.data_ptr(), (t.stride(0) if len(shape) == 2 and shape[0] > 1 else 0), t
 
 
 def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
@@ -263,57 +290,44 @@ def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
             raise ValueError("residual_out must have evenly spaced rows of contiguous features")
         if total.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("residual_out requires a gradient: this operator is inference only")
-    out = _empty_fp8(x.shape, x.device) if out_dtype == torch.float8_e4m3fn \
-        else torch.empty(x.shape, dtype=out_dtype, device=x.device)
     dev = x.device
-    vecs = {n: _vector(n, t, s, dev) for n, t, s in (
-        ("gate", gate, (batch, dim)), ("scale", scale, (batch, dim)), ("shift", shift, (batch, dim)),
-        ("weight", weight, (dim,)), ("bias", bias, (dim,)))}
-    if x.numel() == 0:
-        return out, total
-    a = AddNormArgs()
-    xr, a.x_stride = _rows(x)
-    a.x = xr.data_ptr()
-    if y is not None:
-        yr, a.y_stride = _rows(y)
-        a.y, a.sum, a.sum_stride = yr.data_ptr(), total.data_ptr(), _row_stride(total)
-    for n, (t, s) in vecs.items():
-        if t is not None:
-            setattr(a, n, t.data_ptr())
-            if n in ("gate", "scale", "shift"):
-                setattr(a, n + "_stride", s)
-    if isinstance(out, Fp8Tensor):
-        a.out, a.out_stride = out.data.data_ptr(), _row_stride(out.data)
-        a.out_scale = out.scale.data_ptr()
-        a.out_scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
-        a.out_type = _TYPES[torch.float8_e4m3fn]
+    g, gs, _g = _vector("gate", gate, (batch, dim), dev)
+    sc, scs, _sc = _vector("scale", scale, (batch, dim), dev)
+    sh, shs, _sh = _vector("shift", shift, (batch, dim), dev)
+    w, _, _w = _vector("weight", weight, (dim,), dev)
+    b, _, _b = _vector("bias", bias, (dim,), dev)
+    if out_dtype == torch.float8_e4m3fn:
+        out, ld, ls = _empty_fp8(x.shape, dev)
+        o, os = out.data.data_ptr(), out.scale.data_ptr()
     else:
-        a.out, a.out_stride, a.out_type = out.data_ptr(), dim, _TYPES[torch.bfloat16]
-    a.rows, a.rows_per_batch = batch * x.shape[-2], x.shape[-2]
-    a.dim, a.x_type, a.norm, a.eps = dim, _TYPES[x.dtype], _NORMS[norm], eps
-    _launch("vx_add_norm", a, dev)
+        out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        o, os, ld, ls = out.data_ptr(), None, dim, 0
+    rows = batch * x.shape[-2]
+    if rows == 0:
+        return out, total
+    xr, x_stride = _rows(x)
+    yp = sp = None
+    y_stride = s_stride = 0
+    if y is not None:
+        y, y_stride = _rows(y)
+        yp, sp, s_stride = y.data_ptr(), total.data_ptr(), _row_stride(total)
+    _launch("vx_add_norm", AddNormArgs(
+        xr.data_ptr(), yp, sp, g, w, b, sc, sh, o, os, x_stride, y_stride, s_stride, ld, gs, scs, shs,
+        (1, ls), rows, x.shape[-2], dim, _TYPES[x.dtype], _TYPES[out_dtype], _NORMS[norm], eps), dev)
     return out, total
 
 
-def _fp8_rows(name: str, t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+def _fp8_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """e4m3 rows on 16-byte boundaries (a padded copy where they are not) and
     their stride."""
     s = _row_stride(t)
     k = t.shape[-1]
-    rows = t.numel() // k
-    if s is not None and t.data_ptr() % 16 == 0 and (s % 16 == 0 or rows == 1):
+    if s is not None and t.data_ptr() % 16 == 0 and (s % 16 == 0 or t.numel() == k):
         return t, -(-s // 16) * 16
-    ld = -(-k // 16) * 16
+    rows, ld = t.numel() // k, -(-k // 16) * 16
     buf = torch.empty((rows, ld), dtype=torch.uint8, device=t.device)
     buf[:, :k] = t.reshape(rows, k).view(torch.uint8)
     return buf, ld
-
-
-def _scale_strides(scale: torch.Tensor):
-    """`scale` (..., blocks) as (rows, blocks) and its two strides."""
-    if scale.dim() > 2:
-        scale = scale.flatten(0, -2)
-    return scale, (scale.stride(0), scale.stride(1))
 
 
 def linear_fp8(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -357,31 +371,24 @@ def linear_fp8(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
         raise NotImplementedError(f"activation {activation!r}: None and 'gelu_tanh' are built")
     if out_dtype not in _TYPES:
         raise NotImplementedError(f"out_dtype {out_dtype}: bfloat16, float32 and float8_e4m3fn are built")
-    bias, _ = _vector("bias", bias, (N,), dev)
+    bp, _, _bias = _vector("bias", bias, (N,), dev)
     shape = (*xd.shape[:-1], N)
-    out = _empty_fp8(shape, dev) if out_dtype == torch.float8_e4m3fn \
-        else torch.empty(shape, dtype=out_dtype, device=dev)
-    if xd.numel() == 0:
-        return out
-    a = LinearFp8Args()
-    xd, a.x_stride = _fp8_rows("x", xd)
-    wd, a.w_stride = _fp8_rows("w", wd)
-    xs, a.x_scale_stride[:] = _scale_strides(xs)
-    ws, a.w_scale_stride[:] = _scale_strides(ws)
-    a.x, a.w, a.x_scale, a.w_scale = (t.data_ptr() for t in (xd, wd, xs, ws))
-    a.bias = bias.data_ptr() if bias is not None else None
-    if isinstance(out, Fp8Tensor):
-        a.out, a.out_stride = out.data.data_ptr(), _row_stride(out.data)
-        a.out_scale = out.scale.data_ptr()
-        a.out_scale_stride[:] = (out.scale.stride(-2), out.scale.stride(-1))
+    m = math.prod(shape[:-1])
+    if out_dtype == torch.float8_e4m3fn:
+        out, ld, ls = _empty_fp8(shape, dev)
+        o, os = out.data.data_ptr(), out.scale.data_ptr()
     else:
-        a.out, a.out_stride = out.data_ptr(), N
-    m = 1
-    for n in shape[:-1]:
-        m *= n
-    a.m, a.n, a.k = m, N, K
-    a.out_type, a.activation, a.variant = _TYPES[out_dtype], _ACTS[activation], variant
-    _launch("vx_linear_fp8", a, dev)
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        o, os, ld, ls = out.data_ptr(), None, N, 0
+    if m == 0:
+        return out
+    xd, x_stride = _fp8_rows(xd)
+    wd, w_stride = _fp8_rows(wd)
+    if xs.dim() > 2:
+        xs = xs.flatten(0, -2)
+    _launch("vx_linear_fp8", LinearFp8Args(
+        xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), ws.data_ptr(), bp, o, os, x_stride, w_stride, ld,
+        xs.stride(), ws.stride(), (1, ls), m, N, K, _TYPES[out_dtype], _ACTS[activation], variant), dev)
     return out
 
 
