@@ -50,6 +50,8 @@ struct AddNormParams {
   int dim;
   int layer;                  // 1: LayerNorm, 0: RMSNorm
   float eps;
+  int sum_on16, out_on16;     // rows of the sum / output on 16-byte (e4m3: 8-byte) boundaries
+  int cap;                    // dim rounded up to 256
 };
 
 template <int W>
@@ -89,38 +91,36 @@ __device__ __forceinline__ void affine(const AddNormParams& p, long long bi, int
 }
 
 // The lane's eight values of a chunk of floats in shared memory.
-template <bool kVec>
 __device__ __forceinline__ void smem8(const float* chunk, int lane, float (&f)[8]) {
-  if constexpr (kVec) {
-    const float4 a = reinterpret_cast<const float4*>(chunk)[2 * lane];
-    const float4 b = reinterpret_cast<const float4*>(chunk)[2 * lane + 1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = chunk[i * 32 + lane];
-  }
+  const float4 a = reinterpret_cast<const float4*>(chunk)[2 * lane];
+  const float4 b = reinterpret_cast<const float4*>(chunk)[2 * lane + 1];
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
 template <bool kVec>
 __device__ __forceinline__ void store_out(const AddNormParams& p, long long row, int c0, int lane,
-                                          int n, const float (&o)[8]) {
+                                          int n, const float (&o)[8], void* turn) {
   if (p.out_scale == nullptr)
-    store_chunk<kVec>(static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + c0, lane, n, o);
+    store_chunk<kVec>(static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + c0, lane, n, o,
+                      p.out_on16 != 0, turn);
   else
     quantize_chunk<kVec>(static_cast<uint8_t*>(p.out) + row * p.out_stride + c0,
                          p.out_scale + row * p.out_scale_rs + (c0 / kBlock) * p.out_scale_bs,
-                         p.out_scale_bs, lane, n, o);
+                         p.out_scale_bs, lane, n, o, p.out_on16 != 0);
 }
 
 template <typename T, int W, int NV, bool kVec>
 __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ AddNormParams p) {
   __shared__ float part[8];
+  __shared__ float4 turn_smem[kVec ? 1 : 8 * 64];
   extern __shared__ float4 norm_smem[];
-  constexpr int kCap = 256 * W * NV;  // features the CTA's registers hold
   float* const sa = reinterpret_cast<float*>(norm_smem);
-  float* const sb = sa + kCap;
-  float* const sg = sb + kCap;  // with y only
+  float* const sb = sa + p.cap;
+  float* const sg = sb + p.cap;  // with y only
+  void* const turn = turn_smem + (kVec ? 0 : (threadIdx.x >> 5) * 64);
+  // Narrow rows: the next row's loads start before this one's statistics.
+  constexpr bool kAhead = NV <= 2;
   const int lane = threadIdx.x & 31;
   const int chunk0 = ((threadIdx.x >> 5) & (W - 1)) * 256;  // + 256 W v
   const float inv_n = 1.f / static_cast<float>(p.dim);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ A
   for (long long row0 = blockIdx.x * p.rows_per_cta; row0 < last;) {
     const long long bi = row0 / p.rows_per_batch;
     const long long end = min(last, (bi + 1) * p.rows_per_batch);
-    for (int c = threadIdx.x; c < kCap; c += 256) {  // past the row's end: 0
+    for (int c = threadIdx.x; c < p.cap; c += 256) {  // past the row's end: 0
       float a = 0.f, b = 0.f, g = 0.f;
       if (c < p.dim) {
         affine(p, bi, c, a, b);
@@ -139,44 +139,58 @@ __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ A
       if (p.y != nullptr) sg[c] = g;
     }
     __syncthreads();
-    for (; row0 < end; row0 += 8 / W) {
-      // Rows past the segment's end work on its last row and store nothing,
-      // but stay for the barriers and shuffles.
-      const long long mine = row0 + threadIdx.x / (32 * W);
-      const bool live = mine < end;
-      const long long row = live ? mine : end - 1;
+    // Rows past the segment's end work on its last row and store nothing, but
+    // stay for the barriers and shuffles.
+    Raw<T, kVec> rx[NV];
+    Raw<__nv_bfloat16, kVec> ry[NV];
+    auto load_row = [&](long long r0) {
+      const long long row = min(r0 + threadIdx.x / (32 * W), end - 1);
       const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-      Raw<T, kVec> rx[NV];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c0 = chunk0 + 256 * W * v;
         rx[v].load(x + c0, lane, p.dim - c0);
       }
-      float h[NV][8];
       if (p.y != nullptr) {
         const __nv_bfloat16* y = p.y + row * p.y_stride;
-        Raw<__nv_bfloat16, kVec> ry[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const int c0 = chunk0 + 256 * W * v;
           ry[v].load(y + c0, lane, p.dim - c0);
         }
+      }
+    };
+    if (kAhead) load_row(row0);
+    for (; row0 < end; row0 += 8 / W) {
+      const long long mine = row0 + threadIdx.x / (32 * W);
+      const bool live = mine < end;
+      const long long row = live ? mine : end - 1;
+      if (!kAhead) load_row(row0);
+      float h[NV][8];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) rx[v].get(h[v]);
+      if (p.y != nullptr) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c0 = chunk0 + 256 * W * v;
+          if (c0 >= p.dim) break;  // the warp's remaining chunks lie past the row's end
+          float yv[8], g[8];
+          ry[v].get(yv);
+          smem8(sg + c0, lane, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[v][i] = stored(fmaf(yv[i], g[i], h[v][i]), T());
+        }
+      }
+      // In place, the next rows are other rows: their loads may pass the stores.
+      if (kAhead && row0 + 8 / W < end) load_row(row0 + 8 / W);
+      if (p.y != nullptr) {
         // In place is fine: each lane writes only the features it has read itself.
         T* sum = static_cast<T*>(p.sum) + row * p.sum_stride;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const int c0 = chunk0 + 256 * W * v;
-          float yv[8], g[8];
-          rx[v].get(h[v]);
-          ry[v].get(yv);
-          smem8<kVec>(sg + c0, lane, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) h[v][i] = stored(fmaf(yv[i], g[i], h[v][i]), T());
-          store_chunk<kVec>(sum + c0, lane, live ? p.dim - c0 : 0, h[v]);
+          store_chunk<kVec>(sum + c0, lane, live ? p.dim - c0 : 0, h[v], p.sum_on16 != 0, turn);
         }
-      } else {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) rx[v].get(h[v]);
       }
       float mean = 0.f, s = 0.f;
       if (p.layer) {
@@ -189,11 +203,11 @@ __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ A
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int n = p.dim - (chunk0 + 256 * W * v);
+        const int n = p.dim - (chunk0 + 256 * W * v) - lane * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           h[v][i] -= mean;
-          const float d = feature<kVec>(lane, i) < n ? h[v][i] : 0.f;
+          const float d = i < n ? h[v][i] : 0.f;
           s = fmaf(d, d, s);
         }
       }
@@ -201,12 +215,13 @@ __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ A
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c0 = chunk0 + 256 * W * v;
+        if (c0 >= p.dim) break;
         float a[8], b[8];
-        smem8<kVec>(sa + c0, lane, a);
-        smem8<kVec>(sb + c0, lane, b);
+        smem8(sa + c0, lane, a);
+        smem8(sb + c0, lane, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[v][i] = fmaf(h[v][i] * rstd, a[i], b[i]);
-        store_out<kVec>(p, row, c0, lane, live ? p.dim - c0 : 0, h[v]);
+        store_out<kVec>(p, row, c0, lane, live ? p.dim - c0 : 0, h[v], turn);
       }
     }
     row0 = end;
@@ -217,6 +232,8 @@ __global__ void __launch_bounds__(256) add_norm_kernel(const __grid_constant__ A
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constant__ AddNormParams p) {
   __shared__ float part[8];
+  __shared__ float4 turn_smem[8 * 64];
+  void* const turn = turn_smem + (threadIdx.x >> 5) * 64;
   const int lane = threadIdx.x & 31;
   const int chunk0 = (threadIdx.x >> 5) * 256;
   const long long row = blockIdx.x;
@@ -243,7 +260,8 @@ __global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constan
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         h[i] = stored(p.gate != nullptr ? fmaf(y[i], g[i], h[i]) : h[i] + y[i], T());
-      store_chunk<kVec>(static_cast<T*>(p.sum) + row * p.sum_stride + c0, lane, n, h);
+      store_chunk<kVec>(static_cast<T*>(p.sum) + row * p.sum_stride + c0, lane, n, h,
+                        p.sum_on16 != 0, turn);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -251,7 +269,8 @@ __global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constan
       s2 = fmaf(h[i], h[i], s2);
     }
   }
-  // each lane reads again what it wrote itself
+  // read again below, in rows off the boundaries by other lanes of the warp
+  __syncwarp();
   const T* src = p.y != nullptr ? static_cast<const T*>(p.sum) + row * p.sum_stride : x;
   if (p.layer) {
     mean = row_sum<8>(s, part) * inv_n;
@@ -264,7 +283,7 @@ __global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constan
       rx.get(h);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = feature<kVec>(lane, i) < n ? h[i] - mean : 0.f;
+        const float d = lane * 8 + i < n ? h[i] - mean : 0.f;
         s2 = fmaf(d, d, s2);
       }
     }
@@ -278,12 +297,12 @@ __global__ void __launch_bounds__(256) add_norm_wide_kernel(const __grid_constan
     rx.get(h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = feature<kVec>(lane, i);
+      const int c = lane * 8 + i;
       float a = 0.f, b = 0.f;
       if (c < n) affine(p, bi, c0 + c, a, b);
       h[i] = fmaf((h[i] - mean) * rstd, a, b);
     }
-    store_out<kVec>(p, row, c0, lane, n, h);
+    store_out<kVec>(p, row, c0, lane, n, h, turn);
   }
 }
 

@@ -48,15 +48,13 @@ __device__ __forceinline__ float lanes_max(float m) {
   return m;
 }
 
-// A warp's 256 consecutive features of a row, eight per lane. kVec (rows of
-// 8 k features on 16-byte boundaries): lane l holds features 8 l .. 8 l + 7,
-// moved as vectors; a half-warp then holds one block of 128. Otherwise lane l
-// holds features l, l + 32, ..., so that a warp's element accesses are
-// neighbours; elements 0-3 and 4-7 of all lanes are the two blocks.
-template <bool kVec>
-__device__ __forceinline__ int feature(int lane, int i) {
-  return kVec ? lane * 8 + i : i * 32 + lane;
-}
+// A warp's 256 consecutive features of a row: lane l holds features 8 l ..
+// 8 l + 7, so a half-warp holds one block of 128. kVec: rows of 8 k features
+// on 16-byte boundaries. Any other row (odd widths or strides) is read through
+// the aligned 16-byte pieces that its bytes lie in, shifted into place: a row
+// starts at another offset each time, but the same for all lanes. A piece that
+// holds one of the row's bytes lies in the same page, so nothing outside the
+// caller's memory is touched that could fault.
 
 // The lane's eight elements as they lie in memory (`row` points at the chunk,
 // of which the first `n` features exist; the others read 0).
@@ -93,94 +91,130 @@ struct Raw<__nv_bfloat16, true> {
     }
   }
 };
+// Words w[q ..] of the pieces, q = 0..3.
+template <int N>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[N], uint32_t q) {
+#pragma unroll
+  for (int i = 0; i + 2 < N; ++i) w[i] = q & 2u ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i + 1 < N; ++i) w[i] = q & 1u ? w[i + 1] : w[i];
+}
+__device__ __forceinline__ void put4(uint32_t* w, const uint4& v) {
+  w[0] = v.x;
+  w[1] = v.y;
+  w[2] = v.z;
+  w[3] = v.w;
+}
+// The 16-byte piece `k` after the one that holds `p`, if bytes [16 k, ...) of
+// it are wanted (`bytes` from p on).
+__device__ __forceinline__ uint4 piece(const void* p, int k, int bytes) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (bytes > 0 && static_cast<int>(at & 15u) + bytes > 16 * k)
+    v = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15))[k];
+  return v;
+}
 template <>
 struct Raw<float, false> {
-  float v[8];
+  uint4 a, b, c;
+  uint32_t q;
+  int have;
   __device__ __forceinline__ void load(const float* row, int lane, int n) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = 0.f;
-      if (i * 32 + lane < n) v[i] = row[i * 32 + lane];
-    }
+    const float* p = row + lane * 8;
+    have = n - lane * 8;
+    const int bytes = min(have, 8) * 4;
+    q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u) >> 2;
+    a = piece(p, 0, bytes);
+    b = piece(p, 1, bytes);
+    c = piece(p, 2, bytes);
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
+    uint32_t w[12];
+    put4(w, a);
+    put4(w + 4, b);
+    put4(w + 8, c);
+    shift_words(w, q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = v[i];
+    for (int i = 0; i < 8; ++i) f[i] = i < have ? __uint_as_float(w[i]) : 0.f;
   }
 };
 template <>
 struct Raw<__nv_bfloat16, false> {
-  uint16_t v[8];
+  uint4 a, b;
+  uint32_t at;
+  int have;
   __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane, int n) {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = 0;
-      if (i * 32 + lane < n) v[i] = p[i * 32 + lane];
-    }
+    const __nv_bfloat16* p = row + lane * 8;
+    have = n - lane * 8;
+    const int bytes = min(have, 8) * 2;
+    at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
+    a = piece(p, 0, bytes);
+    b = piece(p, 1, bytes);
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
+    uint32_t w[8];
+    put4(w, a);
+    put4(w + 4, b);
+    shift_words(w, at >> 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(static_cast<uint32_t>(v[i]) << 16);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = __funnelshift_r(w[i], w[i + 1], (at & 2u) * 8u);
+      f[2 * i] = 2 * i < have ? __uint_as_float(v << 16) : 0.f;
+      f[2 * i + 1] = 2 * i + 1 < have ? __uint_as_float(v & 0xffff0000u) : 0.f;
+    }
   }
 };
 
-template <bool kVec>
-__device__ __forceinline__ void store_chunk(float* row, int lane, int n, const float (&f)[8]) {
-  if constexpr (kVec) {
-    if (lane * 8 < n) {
-      reinterpret_cast<float4*>(row)[2 * lane] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(row)[2 * lane + 1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < n) row[i * 32 + lane] = f[i];
-  }
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
-template <bool kVec>
-__device__ __forceinline__ void store_chunk(__nv_bfloat16* row, int lane, int n, const float (&f)[8]) {
-  if constexpr (kVec) {
-    if (lane * 8 < n)
-      reinterpret_cast<uint4*>(row)[lane] =
-          make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                     pack_bf16x2(f[6], f[7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < n) row[i * 32 + lane] = __float2bfloat16(f[i]);
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                            pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
+// Stores the chunk. Rows off the 16-byte boundaries (`on16` false) leave
+// element by element, neighbours by neighbouring lanes, through `turn` (the
+// warp's own 256 elements of shared memory).
+template <bool kVec, typename T>
+__device__ __forceinline__ void store_chunk(T* row, int lane, int n, const float (&f)[8], bool on16,
+                                            void* turn) {
+  if (kVec || (on16 && n >= 256)) {
+    if (lane * 8 < n) store8(row + lane * 8, f);
+    return;
   }
+  T* t = static_cast<T*>(turn);
+  __syncwarp();
+  store8(t + lane * 8, f);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i * 32 + lane < n) row[i * 32 + lane] = t[i * 32 + lane];
 }
 
 // Quantises and stores the chunk (features past the end must be 0); `scale`
 // points at the scale of its first block, the second is `bs` floats on.
+// `on8`: the row lies on an 8-byte boundary.
 template <bool kVec>
 __device__ __forceinline__ void quantize_chunk(uint8_t* row, float* scale, long long bs, int lane,
-                                               int n, const float (&f)[8]) {
-  const float lo = amax4(f[0], f[1], f[2], f[3]), hi = amax4(f[4], f[5], f[6], f[7]);
+                                               int n, const float (&f)[8], bool on8) {
   float inv;
-  if constexpr (kVec) {
-    const float s = block_scale(lanes_max<16>(fmaxf(lo, hi)), inv);
-    if (lane * 8 < n) {
-      reinterpret_cast<uint2*>(row)[lane] =
-          make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                     pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-      if ((lane & 15) == 0) scale[(lane >> 4) * bs] = s;
-    }
+  const float s = block_scale(
+      lanes_max<16>(fmaxf(amax4(f[0], f[1], f[2], f[3]), amax4(f[4], f[5], f[6], f[7]))), inv);
+  const int have = n - lane * 8;
+  if (have <= 0) return;
+  const uint2 q = make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                             pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+  uint8_t* o = row + lane * 8;
+  if (kVec || (on8 && have >= 8)) {
+    *reinterpret_cast<uint2*>(o) = q;
   } else {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const float s = block_scale(lanes_max<32>(half ? hi : lo), inv);
-      const uint32_t q = pack_e4m3x4(f[4 * half] * inv, f[4 * half + 1] * inv,
-                                     f[4 * half + 2] * inv, f[4 * half + 3] * inv);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = (4 * half + i) * 32 + lane;
-        if (c < n) row[c] = static_cast<uint8_t>(q >> (8 * i));
-      }
-      if (lane == 0 && half * kBlock < n) scale[half * bs] = s;
-    }
+    for (int i = 0; i < 8; ++i)
+      if (i < have) o[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
   }
+  if ((lane & 15) == 0) scale[(lane >> 4) * bs] = s;
 }
 
 }  // namespace fp8

@@ -66,21 +66,25 @@ std::map<std::pair<const void*, int>, int> g_norm_ctas;
 template <typename T, int W, int NV, bool kVec>
 int launch_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
   const void* fn = reinterpret_cast<const void*>(&add_norm_kernel<T, W, NV, kVec>);
-  constexpr size_t kFull = 3u * 256 * W * NV * sizeof(float);
-  const size_t smem = p.y != nullptr ? kFull : kFull / 3 * 2;
-  int rc = vx_internal_prepare_kernel(fn, dev, kFull);
+  constexpr size_t kMost = 3u * 256 * W * NV * sizeof(float);
+  p.cap = (p.dim + 255) / 256 * 256;
+  const size_t smem = (p.y != nullptr ? 3u : 2u) * p.cap * sizeof(float);
+  int rc = vx_internal_prepare_kernel(fn, dev, kMost);
   if (rc != VX_OK) return rc;
-  int per_sm;
+  int per_sm;  // by registers and threads
   {
     std::lock_guard<std::mutex> lk(g_norm_mu);
     int& n = g_norm_ctas[{fn, dev}];
     if (n == 0) {
-      cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 256, kFull);
+      cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 256, 0);
       if (e != cudaSuccess) return vx_internal_cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
       n = std::max(n, 1);
     }
     per_sm = n;
   }
+  // and by the 228 KB of shared memory, 1 KB of which each CTA holds besides
+  // its own (and 8 KB where rows lie off the boundaries)
+  per_sm = std::max(1, std::min<int>(per_sm, 228 * 1024 / (smem + 1024 + (kVec ? 64 : 8256))));
   constexpr int kPer = 8 / W;  // rows at a time
   const long long groups = (p.rows + kPer - 1) / kPer;
   const long long ctas = std::min<long long>(groups, static_cast<long long>(sms) * per_sm);
@@ -97,11 +101,14 @@ int launch_add_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
   // each (a row's latency then counts, not its bandwidth).
   const int vecs = (p.dim + 255) / 256;
   const bool few = p.rows < 4LL * sms;
+  // Rows off the 16-byte boundaries hold their pieces (up to 12 registers per
+  // eight features) and the features at once.
+  const int most1 = kVec ? 6 : 4;
   if (vecs <= 1) return launch_norm<T, 1, 1, kVec>(p, dev, sms, s);
-  if (!few) {
+  if (!few && vecs <= most1) {
     if (vecs <= 2) return launch_norm<T, 1, 2, kVec>(p, dev, sms, s);
     if (vecs <= 4) return launch_norm<T, 1, 4, kVec>(p, dev, sms, s);
-    if (vecs <= 6) return launch_norm<T, 1, 6, kVec>(p, dev, sms, s);
+    if constexpr (kVec) return launch_norm<T, 1, 6, kVec>(p, dev, sms, s);
   }
   if (vecs <= 4) return launch_norm<T, 4, 1, kVec>(p, dev, sms, s);
   if (vecs <= 8) return launch_norm<T, 4, 2, kVec>(p, dev, sms, s);
@@ -226,6 +233,7 @@ extern "C" int vx_quantize_fp8(const vx_quantize_fp8_args* a, vx_stream_t stream
   const bool vec =
       a->dim % 8 == 0 && vec8(p.src, p.src_stride, elem) && vec8(p.dst, p.dst_stride, 1);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  p.on8 = vec8(p.dst, p.dst_stride, 1);
   const unsigned grid = by_row ? (p.items + 7) / 8 : p.items;
   if (a->src_type == VX_TYPE_FLOAT) {
     if (!by_row) quantize_tiles_kernel<float><<<grid, 256, 0, s>>>(p);
@@ -304,6 +312,8 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
   p.dim = a->dim;
   p.layer = a->norm == VX_NORM_LAYER;
   p.eps = a->eps;
+  p.sum_on16 = a->y != nullptr && vec8(a->sum, a->sum_stride, xe);
+  p.out_on16 = vec8(a->out, a->out_stride, oe);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a->x_type == VX_TYPE_FLOAT)
     rc = vec ? launch_add_norm<float, true>(p, dev, sms, s) : launch_add_norm<float, false>(p, dev, sms, s);

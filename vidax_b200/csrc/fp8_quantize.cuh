@@ -3,9 +3,7 @@
 // quantize_rows_kernel: blocks of 128 features of one row (activations). A
 //   warp takes 256 features (two blocks) of kRows rows: a block's largest
 //   magnitude is a few shuffles away, the row is read once, and the rows'
-//   loads are all in flight together. Rows that vectors do not fit (odd
-//   widths or strides) are read and written element by element, neighbours by
-//   neighbouring lanes.
+//   loads are all in flight together.
 // quantize_tiles_kernel: 128 x 128 blocks (weights), one block per CTA.
 //
 // Both are bound by HBM: 2 or 4 bytes read, 1 + 4/128 written per element.
@@ -26,6 +24,7 @@ struct QuantizeParams {
   int dim;
   int chunks;        // of 256 features (rows kernel) or 128 (tiles kernel) per row
   unsigned items;    // row groups * chunks
+  int on8;           // the output's rows lie on 8-byte boundaries
 };
 
 constexpr int kRows = 4;
@@ -51,7 +50,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
     const long long r = r0 + i;
     quantize_chunk<kVec>(p.dst + r * p.dst_stride + c0,
                          p.scale + r * p.scale_rs + (c0 / kBlock) * p.scale_bs, p.scale_bs, lane,
-                         i < rows ? n : 0, f);
+                         i < rows ? n : 0, f, p.on8 != 0);
   }
 }
 
