@@ -20,7 +20,10 @@ The projections and FFN are plain bf16 GEMMs (cuBLAS through torch, the
 FFN's bias + tanh-GELU in the cuBLASLt epilogue); the attention, the
 pre-attention step, the Ulysses layout and the block's elementwise glue
 (LayerNorm + modulation + cast, gated residual adds: one pass each) are this
-library's kernels. Weights are random (no checkpoints here), drawn N(0, 0.02) unless
+library's kernels. `quantize_params` gives the blocks' linear layers 8-bit
+weights (vidax_b200.fp8); the forward then runs them on the tensor cores'
+8-bit path, each norm taking in the residual addition before it and handing
+e4m3 activations on. Weights are random (no checkpoints here), drawn N(0, 0.02) unless
 the reference initialises otherwise (modulation tables N(0, dim^-0.5),
 norm3's affine and the RMSNorm scales ones / zeros).
 """
@@ -37,6 +40,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .attention import local_attention
+from .fp8 import Fp8Tensor, add_norm, linear_fp8, quantize_fp8
 from .prologue import attend, rms_norm_rope, rope3d_freqs
 
 
@@ -106,6 +110,26 @@ def init_params(cfg: WanConfig, device, seed: int = 0,
     p["head_w"] = normal(pt * ph * pw * cfg.out_dim, d)
     p["head_b"] = zeros(pt * ph * pw * cfg.out_dim)
     return p
+
+
+def quantize_params(p: Dict[str, torch.Tensor], cfg: WanConfig) -> Dict[str, torch.Tensor]:
+    """`p` with the blocks' linear layers as 8-bit weights: an `Fp8Tensor`
+    (e4m3, a float32 scale per 128 x 128 block) and a float32 bias per layer,
+    self-attention's q, k and v as one layer. `wan_dit_forward` takes either
+    form. Embeddings, modulation, norms and the head keep theirs."""
+    out = {n: t for n, t in p.items() if not n.startswith("blocks_")
+           or not n.endswith(("_w", "_b")) or "norm" in n}
+    for i in range(cfg.num_layers):
+        b = f"blocks_{i}."
+        layers = {f"{a}_{x}": (f"{a}_{x}",) for a in ("self_attn", "cross_attn") for x in "qkvo"}
+        layers.update(ffn_0=("ffn_0",), ffn_2=("ffn_2",))
+        for x in "qkv":
+            del layers[f"self_attn_{x}"]
+        layers["self_attn_qkv"] = tuple(f"self_attn_{x}" for x in "qkv")
+        for name, parts in layers.items():
+            out[b + name + "_w"] = quantize_fp8(torch.cat([p[b + n + "_w"] for n in parts]), 128)
+            out[b + name + "_b"] = torch.cat([p[b + n + "_b"] for n in parts]).float()
+    return out
 
 
 def sinusoidal_embedding_1d(dim: int, position: torch.Tensor) -> torch.Tensor:
@@ -255,6 +279,43 @@ def block_forward(p, i: int, cfg: WanConfig, x, context, t_mod, rope,
     return gated_residual_(x, h, gate_mlp)
 
 
+def _block_forward_fp8(p, i: int, cfg: WanConfig, x, pending, context: Fp8Tensor, t_mod, rope,
+                       sp_axis_name: Optional[str] = None):
+    """`block_forward` with 8-bit linear layers. Every gated residual addition
+    runs inside the norm that follows it, so the last one of a block is handed
+    on: `pending` is the (y, gate) that x still lacks; returns (x, pending)."""
+    b = f"blocks_{i}."
+    d, H = x.shape[-1], cfg.num_heads
+    fp8 = torch.float8_e4m3fn
+    e = p[b + "modulation"] + t_mod.float()
+    shift_msa, scale_msa, gate_msa, shift_mlp, scale_mlp, gate_mlp = (e[:, j] for j in range(6))
+
+    def norm(y, gate, **kw):
+        return add_norm(x, y, gate, norm="layer", eps=cfg.eps, out_dtype=fp8,
+                        residual_out=None if y is None else x, **kw)[0]
+
+    def linear(inp, name, **kw):
+        return linear_fp8(inp, p[b + name + "_w"], p[b + name + "_b"], **kw)
+
+    qkv = linear(norm(*pending, scale=scale_msa, shift=shift_msa), "self_attn_qkv")
+    o = attend(qkv[..., :d], qkv[..., d:2 * d], qkv[..., 2 * d:], H,
+               norm_q=p[b + "self_attn_norm_q"], norm_k=p[b + "self_attn_norm_k"], rope=rope,
+               eps=cfg.eps, sp_axis_name=sp_axis_name)
+    y = linear(quantize_fp8(o), "self_attn_o")
+
+    q = linear(norm(y, gate_msa, weight=p[b + "norm3_w"], bias=p[b + "norm3_b"]), "cross_attn_q")
+    qn = rms_norm_rope(q, p[b + "cross_attn_norm_q"], None, H, eps=cfg.eps)
+    kn = rms_norm_rope(linear(context, "cross_attn_k"), p[b + "cross_attn_norm_k"], None, H,
+                       eps=cfg.eps)
+    v = linear(context, "cross_attn_v")
+    o = local_attention(qn, kn, v.unflatten(-1, (H, cfg.head_dim)))
+    y = linear(quantize_fp8(o.flatten(2)), "cross_attn_o")
+
+    h = linear(norm(y, None, scale=scale_mlp, shift=shift_mlp), "ffn_0", activation="gelu_tanh",
+               out_dtype=fp8)
+    return x, (linear(h, "ffn_2"), gate_mlp)
+
+
 def post_process(p, cfg: WanConfig, x, e, grid, sp_axis_name: Optional[str] = None):
     """WanHead (dit_layers.py:195-217), the sequence all_gather of the ranks'
     token chunks in rank order (dit.py:350-354), unpatchify."""
@@ -279,13 +340,20 @@ def wan_dit_forward(p, cfg: WanConfig, latents: torch.Tensor, t: torch.Tensor,
     """One WanDiT forward (dit.py:364-394): latents (B, T, H, W, in_dim) on
     every rank, t (B,), context (B, L_text, text_dim); returns
     (B, T, H, W, out_dim) on every rank. `rope`: tables of the whole token
-    grid (default: `rope3d_freqs` of the patch grid)."""
+    grid (default: `rope3d_freqs` of the patch grid). `p` from `init_params`,
+    or from `quantize_params` for 8-bit linear layers."""
     if rope is None:
         tp, hp, wp = (latents.shape[1 + i] // cfg.patch_size[i] for i in range(3))
         rope = rope3d_freqs(tp, hp, wp, cfg.head_dim, device=latents.device)
     x, ctx, e0, rope_l, e, grid = pre_process(p, cfg, latents, t, context, rope, sp_axis_name)
-    for i in range(cfg.num_layers):
-        x = block_forward(p, i, cfg, x, ctx, e0, rope_l, sp_axis_name)
+    if isinstance(p["blocks_0.ffn_0_w"], Fp8Tensor):
+        ctx, pending = quantize_fp8(ctx), (None, None)
+        for i in range(cfg.num_layers):
+            x, pending = _block_forward_fp8(p, i, cfg, x, pending, ctx, e0, rope_l, sp_axis_name)
+        gated_residual_(x, *pending)
+    else:
+        for i in range(cfg.num_layers):
+            x = block_forward(p, i, cfg, x, ctx, e0, rope_l, sp_axis_name)
     return post_process(p, cfg, x, e, grid, sp_axis_name)
 
 
