@@ -461,8 +461,8 @@ int vx_add_norm(const vx_add_norm_args* args, vx_stream_t stream);
  * and 128 features, and e4m3 w (n, k), one scale per 128 x 128 block; float32
  * sums; out bf16, float, or e4m3 with a scale per row and 128 columns. x and w
  * start, and their rows lie, on 16-byte boundaries. `variant` 0 picks the
- * kernel by the sizes; 1..4 force a tile (256 x 256 and 256 x 128 on CTA
- * pairs, 128 x 128, 128 x 64), for tuning. */
+ * kernel by the sizes; 1..3 force a tile of 128 rows x 256, 128 or 64 columns,
+ * for tuning. */
 typedef struct vx_linear_fp8_args {
   const void* x;
   const float* x_scale;

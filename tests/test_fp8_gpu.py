@@ -326,13 +326,13 @@ def test_linear_gelu(m, n, k, out):
     _check_linear(x, w, bias, True, got)
 
 
-@pytest.mark.parametrize("variant", [1, 2, 3, 4])
+@pytest.mark.parametrize("variant", [1, 2, 3])
 @pytest.mark.parametrize("m,n,k", [(1, 40, 100), (128, 64, 128), (300, 700, 1000), (2100, 1300, 512)])
 def test_linear_every_variant(m, n, k, variant):
     """Each tile over one and several tiles per CTA, short and full edges."""
     import vidax_b200 as vx
     x, w, bias = _operands(m, n, k, 7 * m + n + k)
-    for out in ("bf16", "f32") + (("fp8",) if variant < 4 else ()):
+    for out in ("bf16", "f32") + (("fp8",) if variant < 3 else ()):
         got = vx.linear_fp8(x, w, bias, out_dtype=OUTS[out], variant=variant)
         _ok()
         _check_linear(x, w, bias, False, got)
@@ -370,7 +370,7 @@ def test_linear_extreme_values():
     data = codes.view(torch.float8_e4m3fn)
     x = vx.Fp8Tensor(data[:m], torch.rand((m, 2), generator=g, device="cuda") * 1e-3)
     w = vx.Fp8Tensor(data[m:], torch.rand((2, 2), generator=g, device="cuda") * 1e3)
-    for v in (0, 1, 4):
+    for v in (0, 1, 3):
         _check_linear(x, w, None, False, vx.linear_fp8(x, w, out_dtype=torch.float32, variant=v))
     z = torch.zeros((130, k), device="cuda")
     z[7, 3] = float("nan")

@@ -7,24 +7,34 @@
 // S_b is an exact-input tensor-core product (tcgen05 kind::f8f6f4, float32
 // accumulator in TMEM); the scales differ from block to block, so each S_b
 // leaves TMEM and is added to a float32 sum in registers. The tensor core
-// works on the next blocks meanwhile: TMEM holds 512 / kBN block products.
+// works on the next block meanwhile: TMEM holds two products of a 256-wide
+// tile, four of the narrower ones.
 //
 // CTA roles: two or four warpgroups each add up their share of the tile's
 // columns (thread = row); of the last warpgroup, the first warp feeds shared
-// memory by TMA, the second and the fourth issue the MMAs, the third
-// fetches the scales (cp.async, any strides) up to 16 blocks ahead: read from
-// global memory where they are used, their latency cost a third of the time
-// of a long sum. CTAs are persistent: each strides
-// over the output tiles, and the roles' barrier phases run on across tiles, so
-// the next tile's loads and products start while the last one is rounded and
-// stored. A finished tile leaves through shared memory by TMA (full 128-byte
-// lines, edges clipped by the tensor map); an output that TMA cannot address
-// is stored element by element.
+// memory by TMA, the second and the fourth issue the MMAs, the third fetches
+// the scales (cp.async, any strides) up to 16 blocks ahead: read from global
+// memory where they are used, their latency cost a third of the time of a long
+// sum. CTAs are persistent: each strides over the output tiles, and the roles'
+// barrier phases run on across tiles, so the next tile's loads and products
+// start while the last one is rounded and stored. A finished tile leaves
+// through shared memory by TMA (full 128-byte lines, edges clipped by the
+// tensor map); an output that TMA cannot address is stored element by element.
 //
-// kCG = 2 pairs two CTAs (cta_group::2) on one 256-row tile: each holds its
-// 128 rows of the activations and half the tile's weight rows, which halves
-// the weight bytes per CTA (32 KB of operands per 128 x 256 x 128 product
-// instead of 48 KB, what L2 can deliver at the e4m3 rate).
+// What bounds it, measured on 9472 x 8960 -> 2048 (183 us, 1900 TFLOP/s, a
+// plain e4m3 product of the library 131 us): the power cap (1000 W, at 1425 of
+// 1965 MHz). Of the time, adding the scaled products is some 30 us and reading
+// them from TMEM 10. A block takes 920 cycles, 512 of them MMAs; the rest is
+// the way from one to the next use of a TMEM buffer (MMA, commit, a look at
+// the barrier of 110 cycles, the read, the hand-back). Taking cycles out of
+// that way lowers the clock instead of the time by now. Pairs of CTAs on one
+// 256 x 256 tile (cta_group::2), which load a third less, ran as fast within
+// 2 %; two CTAs per SM with half of TMEM each, or two sets of warpgroups on
+// tiles in turn, were 25 to 60 % slower.
+//
+// If a wait runs out of its limit, the abort flag is up and every later wait
+// gives up soon: all roles still walk all of their blocks, so that nothing
+// waits for an arrival that does not come, and the output is not valid.
 #pragma once
 
 #include "fp8_common.cuh"
@@ -59,7 +69,7 @@ constexpr int kGroupBlocks = 4;        // of this many blocks each
 constexpr int kScaleSlots = kScaleGroups * kGroupBlocks;
 constexpr int kScaleFloats = 132;      // 128 rows, the warpgroups' weight scales
 
-template <int kCG, int kBN>
+template <int kBN>
 struct LinDims {
   // Warpgroups that add: four for the widest tile (64 columns each), whose two
   // block products in TMEM leave the reader the shortest time; four warps per
@@ -73,7 +83,7 @@ struct LinDims {
   static constexpr int kFeedRegs = kSumWG == 4 ? 32 : 56;
   static constexpr int kSumRegs = kSumWG == 4 ? 112 : 224;
   static constexpr uint32_t kABytes = kLinRows * kBlock;
-  static constexpr uint32_t kBBytes = kBN / kCG * kBlock;
+  static constexpr uint32_t kBBytes = kBN * kBlock;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kStoreBytes = kSumWG * 4 * 4096;   // 32 rows x 128 bytes per warp
   static constexpr uint32_t kBiasBytes = kSumWG * 4 * kCols * 4;
@@ -97,9 +107,8 @@ struct LinDims {
 
 // control block: barriers, then the TMEM address and the abort flag
 enum : int {
-  kLinFull = 0,        // stages: operands landed (kCG = 2: both CTAs', at the leader)
+  kLinFull = 0,        // stages: operands landed
   kLinDone = 8,        // stages: their MMAs are done (the stage is free, the product complete)
-  kLinAccEmpty = 16,   // 4: product read by every adding warp (kCG = 2: both CTAs', at the leader)
   kLinAmax = 24,       // every warpgroup's largest magnitudes are written
   kLinDrain = 26,      // 2: an issuer's MMAs are done (after an abort)
   kLinScaleFull = 28,  // 4: a group's scales landed
@@ -120,11 +129,6 @@ struct Ring {
   }
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 // True in one lane of the (converged) warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t ok;
@@ -133,93 +137,23 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(ok));
   return ok != 0;
 }
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// Relaxed: what it announces is that TMEM has been read (the reads themselves
-// have completed), not a write. A release at cluster scope would wait for
-// every outstanding global load of the thread (measured: half of all stalls).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
-               : "memory");
-}
-
-// 2-D tiled load into this CTA's shared memory; the bytes are counted on `bar`
-// (kCG = 2: the leader CTA's barrier).
-template <int kCG>
+// 2-D tiled load (no multicast) into this CTA's shared memory.
 __device__ __forceinline__ void lin_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x,
                                          int y, uint64_t policy) {
-  if constexpr (kCG == 1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar), "l"(policy)
-        : "memory");
-  } else {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar), "l"(policy)
-        : "memory");
-  }
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
 }
 
-template <int kCG>
 __device__ __forceinline__ void lin_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         uint32_t accumulate) {
-  if constexpr (kCG == 1) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  }
-}
-
-// Arrives on `bar` (kCG = 2: at the same offset in both CTAs) when the MMAs
-// issued so far are complete.
-template <int kCG>
-__device__ __forceinline__ void lin_commit(uint32_t bar) {
-  if constexpr (kCG == 1) {
-    tc_commit(bar);
-  } else {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(bar),
-        "h"(static_cast<uint16_t>(3))
-        : "memory");
-  }
-}
-
-template <int kCG>
-__device__ __forceinline__ void lin_tmem_alloc(uint32_t slot) {
-  if constexpr (kCG == 1) {
-    tmem_alloc(slot, 512);
-    tmem_relinquish();
-  } else {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-}
-template <int kCG>
-__device__ __forceinline__ void lin_tmem_dealloc(uint32_t tmem) {
-  if constexpr (kCG == 1) {
-    tmem_dealloc(tmem, 512);
-  } else {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-  }
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 // kind::f8f6f4 instruction descriptor: e4m3 operands (format 0), K-major,
@@ -228,25 +162,28 @@ __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// x / (1 + exp(-2 u)) = 0.5 x (1 + tanh u), u = sqrt(2 / pi) (x + 0.044715 x^3).
-// The exponent is bounded so that the product of two denominators stays
-// finite: past 2^60 the quotient is below x * 2^-60, as good as 0.
-__device__ __forceinline__ float gelu_exp(float x) {
-  constexpr float kA = -2.f * 0.7978845608028654f * 1.4426950408889634f;
-  const float t = x * fmaf(kA * 0.044715f * x, x, kA);
-  return ex2_approx(fminf(t, 60.f)) + 1.f;
-}
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two elements share one reciprocal: 1/a = b / (a b).
+// x / (1 + exp(-2 u)) = 0.5 x (1 + tanh u), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// Two elements share one reciprocal, 1/a = b / (a b): the special-function
+// unit bounds this step. The exponent is bounded so that the product of the
+// denominators stays finite: past 2^60 the quotient is below x * 2^-60, as
+// good as 0.
 __device__ __forceinline__ void gelu_tanh2(float& x, float& y) {
-  const float a = gelu_exp(x), b = gelu_exp(y);
+  constexpr float kA = -2.f * 0.7978845608028654f * 1.4426950408889634f;
+  const uint64_t v = f2_pack(x, y);
+  const uint64_t t = f2_mul(
+      v, f2_fma(f2_mul(v, v), f2_pack(kA * 0.044715f, kA * 0.044715f), f2_pack(kA, kA)));
+  float t0, t1, a, b;
+  f2_unpack(t, t0, t1);
+  f2_unpack(f2_add(f2_pack(ex2_approx(fminf(t0, 60.f)), ex2_approx(fminf(t1, 60.f))),
+                   f2_pack(1.f, 1.f)),
+            a, b);
   const float r = rcp_approx(a * b);
-  x *= r * b;
-  y *= r * a;
+  f2_unpack(f2_mul(v, f2_pack(r * b, r * a)), x, y);
 }
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
@@ -283,6 +220,19 @@ __device__ __forceinline__ void lin_pack16(const float* v, float inv, uint32_t (
   }
 }
 
+// Hand-over of a TMEM buffer from the sums to an MMA issuer over a named
+// barrier: a look at one in shared memory takes 110 cycles while the tensor
+// core reads its operands. It needs no time limit of its own: every adding
+// warp gets to every block, at the latest when its waits have given up.
+template <int kThreads>
+__device__ __forceinline__ void lin_buffer_arrive(int buf) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(buf + 1), "n"(kThreads) : "memory");
+}
+template <int kThreads>
+__device__ __forceinline__ void lin_buffer_sync(int buf) {
+  asm volatile("bar.sync %0, %1;" ::"r"(buf + 1), "n"(kThreads) : "memory");
+}
+
 // Output tile -> (row tile, column tile): kGroupM row tiles run down before
 // the column advances, so the CTAs at work at one time share both operands
 // through L2.
@@ -295,11 +245,11 @@ __device__ __forceinline__ void lin_tile(const LinearParams& p, int t, int& tm, 
   tm = g * kGroupM + (r - tn * gm);
 }
 
-template <int kCG, int kBN, int kOut>
-__global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
+template <int kBN, int kOut>
+__global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ LinearParams p) {
-  using Dm = LinDims<kCG, kBN>;
+  using Dm = LinDims<kBN>;
   constexpr int S = Dm::kStages, kBufs = Dm::kBufs;
   constexpr int kCols = Dm::kCols;  // columns of a warpgroup
   constexpr int kFeed = 4 * Dm::kSumWG;  // first feeding warp
@@ -313,15 +263,13 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
   // The shuffle tells the compiler that the warp index is the same in all lanes.
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = kCG == 2 ? cluster_rank() : 0u;
-  const int unit0 = blockIdx.x / kCG, unit_step = gridDim.x / kCG;
+  const int unit0 = blockIdx.x, unit_step = gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(bar(kLinFull + i), 1);
       mbar_init(bar(kLinDone + i), 1);
     }
-    for (int i = 0; i < kBufs; ++i) mbar_init(bar(kLinAccEmpty + i), kFeed * kCG);
     for (int i = 0; i < kScaleGroups; ++i) {
       mbar_init(bar(kLinScaleFull + i), 32);
       mbar_init(bar(kLinScaleEmpty + i), kFeed);
@@ -332,14 +280,16 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == kFeed + 1) lin_tmem_alloc<kCG>(sbase + Dm::kCtl + 8 * kLinBars);
+  if (warp == kFeed + 1) {
+    tmem_alloc(sbase + Dm::kCtl + 8 * kLinBars, 512);
+    tmem_relinquish();
+  }
   if (warp == kFeed && lane == 0) {
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_w);
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (kCG == 2) cluster_sync();  // the peer's barriers exist before anything arrives there
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -349,35 +299,26 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
     // ------------------------------------------------------------ producer
     const uint64_t policy = l2_policy_evict_last();
     const bool issuer = elect_one();
-    const uint32_t full0 = kCG == 2 ? map_to_rank(bar(kLinFull), 0) : bar(kLinFull);
     Ring<S> st;
-    int filled = 0;  // stages that have been loaded at least once
-    bool ok = true;
-    for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+    for (int t = unit0; t < p.tiles; t += unit_step) {
       int tm, tn;
       lin_tile(p, t, tm, tn);
-      const int row = (tm * kCG + rank) * kLinRows;
-      const int col = tn * kBN + rank * (kBN / kCG);
+      const int row = tm * kLinRows, col = tn * kBN;
       for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag,
-                                               p.status, kDevTimeoutLoad))) {
-          ok = false;
-          break;
-        }
-        const uint32_t full = full0 + 8u * st.i;
+        mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
         const uint32_t dst = sbase + st.i * Dm::kStageBytes;
         if (issuer) {
-          if (rank == 0) mbar_expect_tx(bar(kLinFull + st.i), kCG * Dm::kStageBytes);
-          lin_load<kCG>(dst, &tm_x, full, kb * kBlock, row, policy);
-          lin_load<kCG>(dst + Dm::kABytes, &tm_w, full, kb * kBlock, col, policy);
+          mbar_expect_tx(bar(kLinFull + st.i), Dm::kStageBytes);
+          lin_load(dst, &tm_x, bar(kLinFull + st.i), kb * kBlock, row, policy);
+          lin_load(dst + Dm::kABytes, &tm_w, bar(kLinFull + st.i), kb * kBlock, col, policy);
         }
-        __syncwarp();
-        if (filled < S) ++filled;
       }
     }
-    if (!ok && rank == 0) {
-      // the loads in flight land before the CTA (pair) gives its memory back
-      for (int i = 0; i < filled; ++i) {
+    if (*abort_flag) {
+      // the loads in flight land before the CTA gives its memory back
+      const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
+      const long long steps = static_cast<long long>(tiles) * p.kblocks;
+      for (int i = 0; i < S && i < steps; ++i) {
         st.i = st.i == 0 ? S - 1 : st.i - 1;
         if (st.i == S - 1) st.phase ^= 1u;
         mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
@@ -385,34 +326,30 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
     }
   } else if (warp == kFeed + 1 || warp == kFeed + 3) {
     // ------------------------------------------------------------ MMA issuers
-    // Two warps take the blocks in turn: a block's two waits, four MMAs and
-    // commit take one issuer 500-600 cycles, a 256 x 256 x 128 product 512 and
-    // the smaller tiles' 256. Blocks are independent (each starts a product),
-    // so tiles do not matter here. The whole warp walks the loop and one lane
-    // issues: addresses and descriptors then stay in uniform registers.
-    if (rank == 0) {
-      constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows * kCG, kBN);
-      const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
-      const bool issuer = elect_one();
-      const int first = warp == kFeed + 3 ? 1 : 0;
-      const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
-      long long left = static_cast<long long>(tiles) * p.kblocks - first;
-      Ring<S> st;
-      Ring<kBufs> ac;
-      if (first) {
-        st.next();
-        ac.next();
-      }
-      bool ok = true;
-      for (; left > 0; left -= 2) {
-        if (!__all_sync(0xffffffffu,
-                        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status,
-                                  kDevTimeoutMma) &&
-                            mbar_wait(bar(kLinAccEmpty + ac.i), ac.phase ^ 1u, abort_flag, p.status,
-                                      kDevTimeoutMma))) {
-          ok = false;
-          break;
-        }
+    // Two warps take the blocks in turn, so that one's waits and issues overlap
+    // the other's. Blocks are independent (each starts a product), so tiles do
+    // not matter here. The whole warp walks the loop and one lane issues:
+    // addresses and descriptors then stay in uniform registers.
+    constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows, kBN);
+    const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
+    const bool issuer = elect_one();
+    const int first = warp == kFeed + 3 ? 1 : 0;
+    const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
+    const long long steps = static_cast<long long>(tiles) * p.kblocks;
+    Ring<S> st;
+    Ring<kBufs> ac;
+    if (first) {
+      st.next();
+      ac.next();
+    }
+    // steps, and then once more for each buffer, so that every arrival of the
+    // sums at the named barriers is met
+    for (long long i = first; i < steps + kBufs; i += 2) {
+      if (i < steps)
+        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
+      if (i >= kBufs && i - kBufs < steps)  // the product before in this buffer has been read
+        lin_buffer_sync<Dm::kSumWG * 128 + 32>(ac.i);
+      if (i < steps) {
         tc_fence_after();
         const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
         const uint64_t db = da + (Dm::kABytes >> 4);
@@ -420,28 +357,26 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
         if (issuer) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
-            lin_mma<kCG>(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
-          lin_commit<kCG>(bar(kLinDone + st.i));
+            lin_mma(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
+          tc_commit(bar(kLinDone + st.i));
         }
-        __syncwarp();
-        st.next();
-        st.next();
-        ac.next();
-        ac.next();
       }
-      if (!ok && issuer) {
-        lin_commit<kCG>(bar(kLinDrain + first));
-        mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
-      }
+      st.next();
+      st.next();
+      ac.next();
+      ac.next();
+    }
+    if (*abort_flag && issuer) {
+      tc_commit(bar(kLinDrain + first));
+      mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
     }
   } else if (warp == kFeed + 2) {
     // ------------------------------------------------------------ scales
     Ring<kScaleGroups> sg;
-    bool ok = true;
-    for (int t = unit0; ok && t < p.tiles; t += unit_step) {
+    for (int t = unit0; t < p.tiles; t += unit_step) {
       int tm, tn;
       lin_tile(p, t, tm, tn);
-      const int row = (tm * kCG + rank) * kLinRows + lane;
+      const int row = tm * kLinRows + lane;
       const int col = tn * kBN + (lane & (Dm::kSumWG - 1)) * kCols;
       const float* xs[4];
 #pragma unroll
@@ -449,11 +384,7 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
         xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
       const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
       for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag,
-                                               p.status, kDevTimeoutLoad))) {
-          ok = false;
-          break;
-        }
+        mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
         const int n = min(kGroupBlocks, p.kblocks - kb0);
         uint32_t dst = sbase + Dm::kScales + sg.i * (kGroupBlocks * kScaleFloats * 4) + lane * 4;
         for (int kb = kb0; kb < kb0 + n; ++kb, dst += kScaleFloats * 4) {
@@ -477,84 +408,82 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
     const float* scale_s = reinterpret_cast<const float*>(smem + Dm::kScales);
     float* bias_s = reinterpret_cast<float*>(smem + Dm::kBias) + warp * kCols;
     float* amax_s = reinterpret_cast<float*>(smem + Dm::kAmax);
-    const uint32_t empty0 = kCG == 2 ? map_to_rank(bar(kLinAccEmpty), 0) : bar(kLinAccEmpty);
     Ring<S> st;
     Ring<kBufs> ac;
     Ring<kScaleGroups> sg;
     uint32_t tile_parity = 0;
-    bool ok = true;
-    for (int t = unit0; ok && t < p.tiles; t += unit_step, tile_parity ^= 1u) {
+    // The bias goes in first. Through shared memory: every lane needs every
+    // column's; a lane fetches its share a tile ahead.
+    auto fetch_bias = [&](int t, float (&v)[kCols / 32]) {
+      int tm = 0, tn = 0;
+      if (t < p.tiles) lin_tile(p, t, tm, tn);
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const int c = tn * kBN + wg * kCols + lane + 32 * i;
+        v[i] = p.bias != nullptr && c < p.n ? p.bias[c] : 0.f;
+      }
+    };
+    float bias[kCols / 32];
+    fetch_bias(unit0, bias);
+    for (int t = unit0; t < p.tiles; t += unit_step, tile_parity ^= 1u) {
       int tm, tn;
       lin_tile(p, t, tm, tn);
-      const int row = (tm * kCG + rank) * kLinRows + r_in;
+      const int row = tm * kLinRows + r_in;
       const int col = tn * kBN + wg * kCols;
       const bool live = row < p.m;
       const int have = p.n - col;  // columns of this warpgroup that exist
-      float bias[kCols / 32];      // of columns col + lane + 32 i
-#pragma unroll
-      for (int i = 0; i < kCols / 32; ++i)
-        bias[i] = p.bias != nullptr && lane + 32 * i < have ? p.bias[col + lane + 32 * i] : 0.f;
       float acc[kCols];
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-      for (int kb = 0; kb < p.kblocks; ++kb, st.next(), ac.next()) {
-        const int in_group = kb % kGroupBlocks;
-        // the warp leaves together: the loads below need all of its lanes
-        if (!__all_sync(0xffffffffu,
-                        (in_group != 0 || mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag,
-                                                    p.status, kDevTimeoutSoftmax)) &&
-                            mbar_wait(bar(kLinDone + st.i), st.phase, abort_flag, p.status,
-                                      kDevTimeoutSoftmax))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t tm_acc = t_lane + ac.i * kBN;
-        uint32_t r[32];
-        tmem_ld32(tm_acc, r);
-        const volatile float* sp = scale_s + (sg.i * kGroupBlocks + in_group) * kScaleFloats;
-        const float sc = sp[r_in] * sp[128 + wg];
-        const uint64_t sc2 = f2_pack(sc, sc);
+      for (int i = 0; i < kCols / 32; ++i) bias_s[lane + 32 * i] = bias[i];
+      __syncwarp();
 #pragma unroll
-        for (int c = 0; c < kCols; c += 32) {
-          if (c > 0) tmem_ld32(tm_acc + c, r);
-          tmem_wait_ld(r);
-          if (c + 32 == kCols) {  // read out: the buffer may take the next product
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (kCG == 2) mbar_arrive_cluster(empty0 + 8u * ac.i);
-              else mbar_arrive(empty0 + 8u * ac.i);
+      for (int j = 0; j < kCols; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias_s + j);
+        acc[j] = b.x;
+        acc[j + 1] = b.y;
+        acc[j + 2] = b.z;
+        acc[j + 3] = b.w;
+      }
+      fetch_bias(t + unit_step, bias);
+      for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
+        mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag, p.status, kDevTimeoutSoftmax);
+        const volatile float* sp = scale_s + sg.i * (kGroupBlocks * kScaleFloats);
+        float sc[kGroupBlocks];  // (of blocks past the last one: not used)
+#pragma unroll
+        for (int g = 0; g < kGroupBlocks; ++g)
+          sc[g] = sp[g * kScaleFloats + r_in] * sp[g * kScaleFloats + 128 + wg];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
+#pragma unroll
+        for (int g = 0; g < kGroupBlocks; ++g) {
+          if (kb0 + g >= p.kblocks) break;
+          mbar_wait(bar(kLinDone + st.i), st.phase, abort_flag, p.status, kDevTimeoutSoftmax);
+          __syncwarp();
+          tc_fence_after();
+          const uint32_t tm_acc = t_lane + ac.i * kBN;
+          const uint64_t sc2 = f2_pack(sc[g], sc[g]);
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(tm_acc + c, r);
+            tmem_wait_ld(r);
+            if (c + 32 == kCols) {  // read out: the buffer may take the next product
+              tc_fence_before();
+              lin_buffer_arrive<Dm::kSumWG * 128 + 32>(ac.i);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const uint64_t v = f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                        sc2, f2_pack(acc[c + j], acc[c + j + 1]));
+              f2_unpack(v, acc[c + j], acc[c + j + 1]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint64_t v = f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), sc2,
-                                      f2_pack(acc[c + j], acc[c + j + 1]));
-            f2_unpack(v, acc[c + j], acc[c + j + 1]);
-          }
-        }
-        if (in_group == kGroupBlocks - 1 || kb + 1 == p.kblocks) {
-          if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
-          sg.next();
+          st.next();
+          ac.next();
         }
       }
-      if (!ok) break;
-      // ---- bias, activation, rounding, store
-      if (p.bias != nullptr) {  // through shared memory: every lane needs every column's
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kCols / 32; ++i) bias_s[lane + 32 * i] = bias[i];
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < kCols; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(bias_s + j);
-          acc[j] += b.x;
-          acc[j + 1] += b.y;
-          acc[j + 2] += b.z;
-          acc[j + 3] += b.w;
-        }
-      }
+      // ---- activation, rounding, store
       if (p.act == kActGeluTanh) {
 #pragma unroll
         for (int j = 0; j < kCols; j += 2) gelu_tanh2(acc[j], acc[j + 1]);
@@ -570,11 +499,7 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
           volatile float* mine = amax_s + tile_parity * (128 * Dm::kSumWG);
           mine[wg * 128 + r_in] = am;
           mbar_arrive(bar(kLinAmax));
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status,
-                                                 kDevTimeoutSoftmax))) {
-            ok = false;
-            break;
-          }
+          mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status, kDevTimeoutSoftmax);
           am = fmaxf(am, mine[(wg ^ 1) * 128 + r_in]);
         }
         const float s = block_scale(am, inv);
@@ -624,11 +549,8 @@ __global__ void __launch_bounds__(LinDims<kCG, kBN>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  // The peer's MMAs read this CTA's shared memory and its arrivals land here:
-  // both stay until both are done.
-  if constexpr (kCG == 2) cluster_sync();
   tc_fence_after();
-  if (warp == kFeed + 1) lin_tmem_dealloc<kCG>(tmem);
+  if (warp == kFeed + 1) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace fp8

@@ -126,74 +126,50 @@ int launch_add_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
 // ------------------------------------------------------------------ linear
 
 struct LinVariant {
-  int cg, bn;
+  int bn;
   const void* fn[3];  // by output type
   uint32_t smem;
   int threads;
   int cols;           // columns of one warpgroup
+  double block, tile; // time model: cycles per block of 128 features, per tile besides
 };
 
-template <int kCG, int kBN>
-LinVariant variant() {
-  return {kCG, kBN,
-          {reinterpret_cast<const void*>(&linear_kernel<kCG, kBN, kOutBf16>),
-           reinterpret_cast<const void*>(&linear_kernel<kCG, kBN, kOutFloat>),
+template <int kBN>
+LinVariant variant(double block, double tile) {
+  return {kBN,
+          {reinterpret_cast<const void*>(&linear_kernel<kBN, kOutBf16>),
+           reinterpret_cast<const void*>(&linear_kernel<kBN, kOutFloat>),
            // a 128-column block of the e4m3 output lies in one tile
            kBN >= kBlock ? reinterpret_cast<const void*>(
-                               &linear_kernel<kCG, (kBN >= kBlock ? kBN : kBlock), kOutE4m3>)
+                               &linear_kernel<(kBN >= kBlock ? kBN : kBlock), kOutE4m3>)
                          : nullptr},
-          LinDims<kCG, kBN>::kSmemBytes,
-          LinDims<kCG, kBN>::kThreads,
-          LinDims<kCG, kBN>::kCols};
+          LinDims<kBN>::kSmemBytes,
+          LinDims<kBN>::kThreads,
+          LinDims<kBN>::kCols,
+          block,
+          tile};
 }
 
-const LinVariant kVariants[] = {variant<2, 256>(), variant<2, 128>(), variant<1, 128>(),
-                                variant<1, 64>()};
+// Measured: 9472 x 8960 -> 2048 takes 922 / 566 / 425 cycles per block, and a
+// tile's start and output 2500 / 2000 / 2000 besides.
+const LinVariant kVariants[] = {variant<256>(922, 2500), variant<128>(566, 2000),
+                                variant<64>(425, 2000)};
+constexpr int kNumVariants = sizeof(kVariants) / sizeof(kVariants[0]);
 
-std::mutex g_lin_mu;
-std::map<std::pair<const void*, int>, int> g_lin_clusters;
-
-// CTA groups of a variant that are resident at once (GPCs with an odd SM
-// count leave an SM without a partner).
-int resident_groups(const LinVariant& v, const void* fn, int dev, int sms, int* out) {
-  if (v.cg == 1) {
-    *out = sms;
-    return VX_OK;
-  }
-  std::lock_guard<std::mutex> lk(g_lin_mu);
-  int& n = g_lin_clusters[{fn, dev}];
-  if (n == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms / 2 * 2);
-    cfg.blockDim = dim3(v.threads);
-    cfg.dynamicSmemBytes = v.smem;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    int got = 0;
-    cudaError_t e = cudaOccupancyMaxActiveClusters(&got, fn, &cfg);
-    if (e != cudaSuccess) return vx_internal_cuda_fail(e, "cudaOccupancyMaxActiveClusters");
-    if (got < 1) return fail(VX_ECUDA, "no cluster of 2 CTAs fits this device");
-    n = got;
-  }
-  *out = n;
-  return VX_OK;
-}
-
+// The tile whose waves over the SMs take least by the time model: narrow ones
+// where wide ones would leave SMs idle.
 int pick_variant(const vx_linear_fp8_args* a, int sms) {
   int best = 0;
-  double best_t = 1e30;
-  for (int i = 0; i < 4; ++i) {
+  double best_t = 0;
+  for (int i = 0; i < kNumVariants; ++i) {
     const LinVariant& v = kVariants[i];
-    if (v.fn[a->out_type == VX_TYPE_E4M3 ? 2 : 0] == nullptr) continue;
-    const long long tiles = ((a->m + v.cg * kLinRows - 1) / (v.cg * kLinRows)) *
-                            static_cast<long long>((a->n + v.bn - 1) / v.bn);
-    const long long groups = sms / v.cg;
-    const double t = static_cast<double>((tiles + groups - 1) / groups) * (v.bn + 64);
-    if (t < best_t) best_t = t, best = i;
+    if (a->out_type == VX_TYPE_E4M3 && v.fn[kOutE4m3] == nullptr) continue;
+    const long long tiles =
+        ((a->m - 1LL) / kLinRows + 1) * ((a->n - 1LL) / v.bn + 1);
+    const double t =
+        static_cast<double>((tiles - 1) / sms + 1) * ((a->k - 1) / kBlock + 1) * v.block +
+        static_cast<double>((tiles - 1) / sms + 1) * v.tile;
+    if (i == 0 || t < best_t) best_t = t, best = i;
   }
   return best;
 }
@@ -335,7 +311,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   if (out_idx < 0) return fail(VX_EUNSUPPORTED, "out_type %d", a->out_type);
   if (a->activation != VX_ACT_NONE && a->activation != VX_ACT_GELU_TANH)
     return fail(VX_EUNSUPPORTED, "activation %d", a->activation);
-  if (a->variant < 0 || a->variant > 4) return fail(VX_EINVAL, "variant %d", a->variant);
+  if (a->variant < 0 || a->variant > kNumVariants) return fail(VX_EINVAL, "variant %d", a->variant);
   if (a->m == 0) return VX_OK;
   int rc;
   if ((rc = check_rows("x", a->x, a->x_stride, a->m, a->k, 1)) != VX_OK) return rc;
@@ -373,7 +349,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   p.m = a->m;
   p.n = a->n;
   p.kblocks = (a->k - 1) / kBlock + 1;
-  p.tiles_m = (a->m - 1) / (v.cg * kLinRows) + 1;
+  p.tiles_m = (a->m - 1) / kLinRows + 1;
   p.tiles_n = (a->n - 1) / v.bn + 1;
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   if (tiles > INT_MAX / 2 || static_cast<long long>(kGroupM) * p.tiles_n > INT_MAX)
@@ -389,7 +365,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   CUtensorMap tx, tw, to;
   if ((rc = vx_internal_byte_tmap(&tx, a->x, a->k, a->m, xst, 128, kLinRows)) != VX_OK) return rc;
-  if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, 128, v.bn / v.cg)) != VX_OK) return rc;
+  if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, 128, v.bn)) != VX_OK) return rc;
   to = tx;  // not used without tma_out
   if (p.tma_out) {
     const uint64_t row = static_cast<uint64_t>(a->n) * oe;
@@ -399,22 +375,9 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
       return rc;
   }
   if ((rc = vx_internal_prepare_kernel(fn, dev, v.smem)) != VX_OK) return rc;
-  int groups;
-  if ((rc = resident_groups(v, fn, dev, sms, &groups)) != VX_OK) return rc;
-
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tiles, groups)) * v.cg);
-  cfg.blockDim = dim3(v.threads);
-  cfg.dynamicSmemBytes = v.smem;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = v.cg;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   void* args[4] = {&tx, &tw, &to, &p};
-  cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  cudaError_t e = cudaLaunchKernel(fn, dim3(static_cast<unsigned>(std::min(p.tiles, sms))),
+                                   dim3(v.threads), args, v.smem, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) {
     cudaGetLastError();
     return vx_internal_cuda_fail(e, "linear_fp8 launch");
