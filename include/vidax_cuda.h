@@ -462,7 +462,7 @@ int vx_add_norm(const vx_add_norm_args* args, vx_stream_t stream);
  * sums; out bf16, float, or e4m3 with a scale per row and 128 columns. x and w
  * start, and their rows lie, on 16-byte boundaries. `variant` 0 picks the
  * kernel by the sizes; 1..3 force a tile of 128 rows x 256, 128 or 64 columns,
- * for tuning. */
+ * 4 the form for up to 16 rows, for tuning. */
 typedef struct vx_linear_fp8_args {
   const void* x;
   const float* x_scale;

@@ -133,7 +133,8 @@ LOK = dict(x=P, x_scale=P, w=P, w_scale=P, out=P, out_scale=P, x_stride=96, w_st
 
 @pytest.mark.parametrize("change,code", [
     (dict(m=-1), 1), (dict(n=0), 1), (dict(k=0), 1), (dict(out_type=3), 2), (dict(activation=2), 2),
-    (dict(variant=-1), 1), (dict(variant=99), 1), (dict(x=None), 1), (dict(w=None), 1),
+    (dict(variant=-1), 1), (dict(variant=99), 1),
+    (dict(variant=4, m=17), 2), (dict(variant=3, out_type=2), 2), (dict(x=None), 1), (dict(w=None), 1),
     (dict(out=None), 1), (dict(x_scale=None), 1), (dict(w_scale=None), 1),
     (dict(out_type=2, out_scale=None), 1), (dict(x=P + 8), 1), (dict(w_stride=100), 1),
     (dict(x_stride=80), 1), (dict(out_stride=63), 1), (dict(bias=P + 1), 1),

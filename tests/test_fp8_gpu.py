@@ -338,6 +338,35 @@ def test_linear_every_variant(m, n, k, variant):
         _check_linear(x, w, bias, False, got)
 
 
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("out", list(OUTS))
+@pytest.mark.parametrize("m", [1, 2, 8, 9, 15, 16])
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 17), (100, 130), (640, 128), (1000, 1187), (257, 4100)])
+def test_linear_few_rows(m, n, k, out, gelu):
+    """The form for a few rows over its token counts, short last blocks of
+    features and of columns, and (n = 1000: 63 CTAs) a last cluster with CTAs
+    that have no column."""
+    import vidax_b200 as vx
+    x, w, bias = _operands(m, n, k, m + 3 * n + k)
+    got = vx.linear_fp8(x, w, bias, activation="gelu_tanh" if gelu else None, out_dtype=OUTS[out],
+                        variant=4)
+    _ok()
+    _check_linear(x, w, bias, gelu, got)
+
+
+def test_linear_padding_behind_the_features_is_not_read_as_values():
+    """NaN codes in the storage behind each row's features."""
+    import vidax_b200 as vx
+    for m, v in ((5, 4), (5, 3), (200, 1)):
+        x, w, bias = _operands(m, 70, 133, 40 + m)
+        ref = vx.linear_fp8(x, w, bias, variant=v)
+        for t in (x, w):
+            full = torch.as_strided(t.data.view(torch.uint8), (t.data.shape[0] - 1, 144), (144, 1))
+            full[:, 133:] = 0x7F
+        assert torch.equal(vx.linear_fp8(x, w, bias, variant=v), ref)
+    _ok()
+
+
 def test_linear_no_bias_batched_and_any_layout():
     import vidax_b200 as vx
     x, w, _ = _operands(6 * 7, 96, 200, 5)
@@ -411,6 +440,25 @@ def test_linear_repeats_bit_for_bit():
     ref = vx.linear_fp8(x, w, bias, out_dtype=torch.float32)
     for _ in range(5):
         assert torch.equal(vx.linear_fp8(x, w, bias, out_dtype=torch.float32), ref)
+
+
+@pytest.mark.parametrize("variant,m,n,k", [(1, 4680, 1024, 1536), (2, 2000, 1024, 1300),
+                                           (3, 1000, 1500, 1536), (4, 8, 4000, 1536)])
+def test_linear_cold_operands(variant, m, n, k):
+    """Operands that come from HBM: their loads land late and out of order.
+    Three sets in turn, and a buffer larger than L2 written in between."""
+    import vidax_b200 as vx
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    sets = [_operands(m, n, k, 50 + i) for i in range(3)]
+    refs = [vx.linear_fp8(*s, out_dtype=torch.float32, variant=variant) for s in sets]
+    _check_linear(*sets[0], False, refs[0])
+    same = []
+    for i in range(60):
+        flush.fill_(i)
+        out = vx.linear_fp8(*sets[i % 3], out_dtype=torch.float32, variant=variant)
+        same.append((out == refs[i % 3]).all())
+    _ok()
+    assert bool(torch.stack(same).all())
 
 
 # ------------------------------------------------------------------ together

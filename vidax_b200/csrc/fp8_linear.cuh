@@ -345,11 +345,17 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
     // steps, and then once more for each buffer, so that every arrival of the
     // sums at the named barriers is met
     for (long long i = first; i < steps + kBufs; i += 2) {
-      if (i < steps)
-        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
       if (i >= kBufs && i - kBufs < steps)  // the product before in this buffer has been read
         lin_buffer_sync<Dm::kSumWG * 128 + 32>(ac.i);
       if (i < steps) {
+        // Only after that: an issuer sees every other block, and with an odd
+        // number of stages the stage's last round was the other issuer's. A
+        // wait tells odd rounds from even ones only, so a look while that
+        // round's load (block i - kStages) is under way would pass. Once block
+        // i - kBufs has been added, so has the one before it in this stage
+        // (kBufs < kStages).
+        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
+        __syncwarp();
         tc_fence_after();
         const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
         const uint64_t db = da + (Dm::kABytes >> 4);
@@ -361,6 +367,7 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           tc_commit(bar(kLinDone + st.i));
         }
       }
+      __syncwarp();
       st.next();
       st.next();
       ac.next();

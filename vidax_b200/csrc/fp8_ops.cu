@@ -13,6 +13,7 @@
 
 #include "add_norm.cuh"
 #include "fp8_linear.cuh"
+#include "fp8_linear_few.cuh"
 #include "fp8_quantize.cuh"
 
 namespace {
@@ -174,6 +175,47 @@ int pick_variant(const vx_linear_fp8_args* a, int sms) {
   return best;
 }
 
+template <int kWarps, int kNT>
+const void* few_kernel(int out) {
+  return out == kOutBf16  ? reinterpret_cast<const void*>(&linear_few_kernel<kWarps, kNT, kOutBf16>)
+         : out == kOutFloat ? reinterpret_cast<const void*>(&linear_few_kernel<kWarps, kNT, kOutFloat>)
+                            : reinterpret_cast<const void*>(&linear_few_kernel<kWarps, kNT, kOutE4m3>);
+}
+
+// Warps share the input features: more of them where few CTAs would leave too
+// few loads in flight.
+bool few_wide(int n, int kblocks, int sms) {
+  return (n - 1) / kFewCols + 1 < 2LL * sms && kblocks > 8;
+}
+
+int launch_few(const FewParams& p, int out, int sms, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  long long ctas = (p.l.n - 1) / kFewCols + 1;
+  const bool wide = few_wide(p.l.n, p.l.kblocks, sms);
+  const void* fn = p.l.m <= 8 ? (wide ? few_kernel<16, 1>(out) : few_kernel<8, 1>(out))
+                              : (wide ? few_kernel<16, 2>(out) : few_kernel<8, 2>(out));
+  cudaLaunchAttribute at[1];
+  if (out == kOutE4m3) {  // the CTAs of one block of 128 output features
+    constexpr int kPeers = kBlock / kFewCols;
+    ctas = (ctas + kPeers - 1) / kPeers * kPeers;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = kPeers;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(wide ? 512 : 256);
+  cfg.stream = stream;
+  void* args[1] = {const_cast<FewParams*>(&p)};
+  cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return vx_internal_cuda_fail(e, "linear_fp8 launch");
+  }
+  return VX_OK;
+}
+
 }  // namespace
 
 extern "C" int vx_quantize_fp8(const vx_quantize_fp8_args* a, vx_stream_t stream) {
@@ -311,7 +353,12 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   if (out_idx < 0) return fail(VX_EUNSUPPORTED, "out_type %d", a->out_type);
   if (a->activation != VX_ACT_NONE && a->activation != VX_ACT_GELU_TANH)
     return fail(VX_EUNSUPPORTED, "activation %d", a->activation);
-  if (a->variant < 0 || a->variant > kNumVariants) return fail(VX_EINVAL, "variant %d", a->variant);
+  if (a->variant < 0 || a->variant > kNumVariants + 1) return fail(VX_EINVAL, "variant %d", a->variant);
+  bool few = a->variant == kNumVariants + 1;
+  if (few && a->m > kFewMost)
+    return fail(VX_EUNSUPPORTED, "this variant takes up to %d rows", kFewMost);
+  if (!few && a->variant > 0 && kVariants[a->variant - 1].fn[out_idx] == nullptr)
+    return fail(VX_EUNSUPPORTED, "this variant has no e4m3 output");
   if (a->m == 0) return VX_OK;
   int rc;
   if ((rc = check_rows("x", a->x, a->x_stride, a->m, a->k, 1)) != VX_OK) return rc;
@@ -329,10 +376,6 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
     return fail(VX_EINVAL, "bias is not aligned to its element");
   int dev, sms;
   if ((rc = vx_internal_device(&dev, &sms)) != VX_OK) return rc;
-  const LinVariant& v = kVariants[a->variant > 0 ? a->variant - 1 : pick_variant(a, sms)];
-  const void* fn = v.fn[out_idx];
-  if (fn == nullptr) return fail(VX_EUNSUPPORTED, "this variant has no e4m3 output");
-
   LinearParams p{};
   p.xs = a->x_scale;
   p.xs_rs = a->x_scale_stride[0];
@@ -349,20 +392,30 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   p.m = a->m;
   p.n = a->n;
   p.kblocks = (a->k - 1) / kBlock + 1;
+  p.act = a->activation;
+  // One row needs no stride; the kernels want one that is a multiple of 16.
+  const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
+  const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
+  if (a->variant == 0)  // (measured: fp8_linear_few.cuh)
+    few = a->m <= 8 || (a->m <= kFewMost && few_wide(a->n, p.kblocks, sms));
+  if (few) {
+    FewParams f{static_cast<const uint8_t*>(a->x), static_cast<const uint8_t*>(a->w),
+                static_cast<long long>(xst), static_cast<long long>(wst), a->k, p};
+    return launch_few(f, out_idx, sms, reinterpret_cast<cudaStream_t>(stream));
+  }
+
+  const LinVariant& v = kVariants[a->variant > 0 ? a->variant - 1 : pick_variant(a, sms)];
+  const void* fn = v.fn[out_idx];
   p.tiles_m = (a->m - 1) / kLinRows + 1;
   p.tiles_n = (a->n - 1) / v.bn + 1;
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   if (tiles > INT_MAX / 2 || static_cast<long long>(kGroupM) * p.tiles_n > INT_MAX)
     return fail(VX_EUNSUPPORTED, "too many output tiles (%lld)", tiles);
   p.tiles = static_cast<int>(tiles);
-  p.act = a->activation;
   const int oe = type_size(a->out_type);
   p.tma_out = aligned(a->out, 16) && a->out_stride * oe % 16 == 0;
   if ((rc = vx_internal_status_word(&p.status)) != VX_OK) return rc;
 
-  // One row needs no stride; the map wants one that is a multiple of 16.
-  const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
-  const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   CUtensorMap tx, tw, to;
   if ((rc = vx_internal_byte_tmap(&tx, a->x, a->k, a->m, xst, 128, kLinRows)) != VX_OK) return rc;
   if ((rc = vx_internal_byte_tmap(&tw, a->w, a->k, a->n, wst, 128, v.bn)) != VX_OK) return rc;
