@@ -75,6 +75,21 @@ def test_python_refusals():
         vx.linear_fp8(q, q)
 
 
+def test_packed_arguments_are_the_structs():
+    """The layouts that the entry points pack their arguments in."""
+    from vidax_b200 import fp8
+    for name, cls in (("vx_quantize_fp8", fp8.QuantizeFp8Args), ("vx_add_norm", fp8.AddNormArgs),
+                      ("vx_linear_fp8", fp8.LinearFp8Args)):
+        flat, values = [], []
+        for n, t in cls._fields_:
+            flat += [(n, i) for i in range(t._length_)] if hasattr(t, "_length_") else [(n, None)]
+        values = list(range(1, len(flat) + 1))
+        raw = fp8._PACKED[name].pack(*values)
+        assert len(raw) == ctypes.sizeof(cls)
+        a = cls.from_buffer_copy(raw)
+        assert [getattr(a, n) if i is None else getattr(a, n)[i] for n, i in flat] == values
+
+
 def _args(cls, **kw):
     a = cls()
     for k, v in kw.items():
