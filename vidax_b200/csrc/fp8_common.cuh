@@ -193,15 +193,16 @@ __device__ __forceinline__ void store_chunk(T* row, int lane, int n, const float
     if (i * 32 + lane < n) row[i * 32 + lane] = t[i * 32 + lane];
 }
 
-// Quantises and stores the chunk (features past the end must be 0); `scale`
-// points at the scale of its first block, the second is `bs` floats on.
-// `on8`: the row lies on an 8-byte boundary.
+// Largest magnitude of the lane's block (a half-warp's chunk of 128 features).
+__device__ __forceinline__ float block_amax(const float (&f)[8]) {
+  return lanes_max<16>(fmaxf(amax4(f[0], f[1], f[2], f[3]), amax4(f[4], f[5], f[6], f[7])));
+}
+
+// The lane's eight features times `inv`, as e4m3 at their place in the chunk
+// (of which `n` features exist). `on8`: the row lies on an 8-byte boundary.
 template <bool kVec>
-__device__ __forceinline__ void quantize_chunk(uint8_t* row, float* scale, long long bs, int lane,
-                                               int n, const float (&f)[8], bool on8) {
-  float inv;
-  const float s = block_scale(
-      lanes_max<16>(fmaxf(amax4(f[0], f[1], f[2], f[3]), amax4(f[4], f[5], f[6], f[7]))), inv);
+__device__ __forceinline__ void store_e4m3(uint8_t* row, int lane, int n, const float (&f)[8],
+                                           float inv, bool on8) {
   const int have = n - lane * 8;
   if (have <= 0) return;
   const uint2 q = make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
@@ -214,7 +215,17 @@ __device__ __forceinline__ void quantize_chunk(uint8_t* row, float* scale, long 
     for (int i = 0; i < 8; ++i)
       if (i < have) o[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
   }
-  if ((lane & 15) == 0) scale[(lane >> 4) * bs] = s;
+}
+
+// Quantises and stores the chunk (features past the end must be 0); `scale`
+// points at the scale of its first block, the second is `bs` floats on.
+template <bool kVec>
+__device__ __forceinline__ void quantize_chunk(uint8_t* row, float* scale, long long bs, int lane,
+                                               int n, const float (&f)[8], bool on8) {
+  float inv;
+  const float s = block_scale(block_amax(f), inv);
+  store_e4m3<kVec>(row, lane, n, f, inv, on8);
+  if ((lane & 15) == 0 && lane * 8 < n) scale[(lane >> 4) * bs] = s;
 }
 
 }  // namespace fp8

@@ -355,7 +355,6 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
         // i - kBufs has been added, so has the one before it in this stage
         // (kBufs < kStages).
         mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
-        __syncwarp();
         tc_fence_after();
         const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
         const uint64_t db = da + (Dm::kABytes >> 4);
@@ -367,7 +366,7 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           tc_commit(bar(kLinDone + st.i));
         }
       }
-      __syncwarp();
+      __syncwarp();  // the named barrier wants the warp together
       st.next();
       st.next();
       ac.next();

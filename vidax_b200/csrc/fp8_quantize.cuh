@@ -43,14 +43,26 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constan
 #pragma unroll
   for (int i = 0; i < kRows; ++i)  // rows past the end: the last one again, not stored
     raw[i].load(static_cast<const T*>(p.src) + (r0 + min(i, rows - 1)) * p.src_stride + c0, lane, n);
+  float f[kRows][8];
+  // Lane i of a half-warp divides for row i % 4 and stores its scale; the rows
+  // then take the factor from that lane.
+  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    float f[8];
-    raw[i].get(f);
-    const long long r = r0 + i;
-    quantize_chunk<kVec>(p.dst + r * p.dst_stride + c0,
-                         p.scale + r * p.scale_rs + (c0 / kBlock) * p.scale_bs, p.scale_bs, lane,
-                         i < rows ? n : 0, f, p.on8 != 0);
+    raw[i].get(f[i]);
+    const float a = block_amax(f[i]);
+    if ((lane & (kRows - 1)) == i) m = a;
+  }
+  float inv;
+  const float s = block_scale(m, inv);
+  const int row = lane & 15, half = lane >> 4;
+  if (row < rows && half * kBlock < n)
+    p.scale[(r0 + row) * p.scale_rs + (c0 / kBlock + half) * p.scale_bs] = s;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const float v = __shfl_sync(0xffffffffu, inv, (lane & 16) + i);
+    store_e4m3<kVec>(p.dst + (r0 + i) * p.dst_stride + c0, lane, i < rows ? n : 0, f[i], v,
+                     p.on8 != 0);
   }
 }
 
