@@ -242,6 +242,34 @@ def test_add_norm_in_place_strided_and_misaligned():
     assert torch.equal(t2, tref) and torch.equal(o2, ref)
 
 
+def test_add_norm_refuses_overlapping_sums():
+    import vidax_b200 as vx
+    buf = torch.zeros((5, 64), device="cuda")
+    y = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="apart"):
+        vx.add_norm(buf[:4], y, residual_out=buf[1:])
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="apart"):
+        vx.add_norm(x, y, residual_out=y)
+    with pytest.raises(ValueError, match="evenly"):
+        vx.add_norm(buf[:4], y, residual_out=torch.zeros((64, 4), device="cuda").t())
+    with pytest.raises(ValueError):
+        vx.add_norm(buf[:4], None, residual_out=buf[:4])
+    with pytest.raises(NotImplementedError, match="gradient"):
+        vx.add_norm(buf[:4], y, weight=torch.ones(64, device="cuda", requires_grad=True))
+    with pytest.raises(ValueError, match="weight"):
+        vx.add_norm(buf[:4], y, weight=torch.ones(63, device="cuda"))
+
+
+def test_add_norm_many_batch_items_of_one_row():
+    """A CTA's run of rows crosses a batch item at every row."""
+    import vidax_b200 as vx
+    c = _norm_case(1500, 1, 384, torch.float32, 15)
+    o, total = vx.add_norm(**c, norm="layer", out_dtype=torch.float8_e4m3fn)
+    _ok()
+    _check_norm(c, "layer", o, total)
+
+
 def test_add_norm_large_mean_keeps_its_variance():
     """LayerNorm of rows with a mean 1000 times their deviation: E[h^2] - m^2
     in float32 would lose the variance."""
@@ -449,6 +477,19 @@ def test_linear_repeats_bit_for_bit():
         assert torch.equal(vx.linear_fp8(x, w, bias, out_dtype=torch.float32), ref)
 
 
+@pytest.mark.parametrize("variant", [1, 2, 3])
+@pytest.mark.parametrize("k", [64, 200, 300, 640])
+def test_linear_few_blocks_many_tiles(k, variant):
+    """One to five blocks of features per tile and several tiles per CTA: the
+    rings of stages, TMEM buffers and scale groups wrap inside and across tiles."""
+    import vidax_b200 as vx
+    x, w, bias = _operands(9000, 700, k, 60 + k)
+    for out in ("f32",) + (("fp8",) if variant < 3 else ()):
+        got = vx.linear_fp8(x, w, bias, out_dtype=OUTS[out], variant=variant)
+        _ok()
+        _check_linear(x, w, bias, False, got)
+
+
 @pytest.mark.parametrize("variant,m,n,k", [(1, 4680, 1024, 1536), (2, 2000, 1024, 1300),
                                            (3, 1000, 1500, 1536), (4, 8, 4000, 1536)])
 def test_linear_cold_operands(variant, m, n, k):
@@ -538,3 +579,35 @@ def test_feed_forward_on_streams_and_in_graphs():
     ref = _layer(new["x"], new["y"], cs[0]["gate"], p)[0]
     _ok()
     assert torch.equal(o, ref)
+
+
+def test_single_token_run_in_a_graph():
+    """One token through norm, up and down projection (the forms for few rows,
+    the e4m3 one a cluster launch), captured and replayed."""
+    p = _layer_params(1536, 2048, 23)
+    c = _norm_case(1, 1, 1536, torch.float32, 34)
+    _layer(c["x"], c["y"], c["gate"], p)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    x = c["x"].clone()
+    with torch.cuda.graph(g):
+        o, _ = _layer(x, c["y"], c["gate"], p)
+    new = _norm_case(1, 1, 1536, torch.float32, 35)
+    x.copy_(new["x"])
+    g.replay()
+    ref, _ = _layer(new["x"], c["y"], c["gate"], p)
+    _ok()
+    assert torch.equal(o, ref)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs 2 GPUs")
+def test_on_another_device_than_the_current_one():
+    p = _layer_params(256, 384, 24)
+    c = _norm_case(1, 40, 256, torch.float32, 36)
+    ref, _ = _layer(c["x"], c["y"], c["gate"], p)
+    import vidax_b200 as vx
+    there = {k: vx.Fp8Tensor(*(t.to("cuda:1") for t in v)) if isinstance(v, tuple) else v.to("cuda:1")
+             for k, v in p.items()}
+    o, _ = _layer(*(c[k].to("cuda:1") for k in ("x", "y", "gate")), there)
+    torch.cuda.synchronize(1)
+    assert torch.equal(o.cpu(), ref.cpu())

@@ -169,6 +169,14 @@ def _row_stride(t: torch.Tensor) -> Optional[int]:
     return stride if stride >= k else None
 
 
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """The addresses that a tensor's elements lie between."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.nbytes
+    return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """`t` (a copy where its rows are not evenly spaced) and its row stride."""
     s = _row_stride(t)
@@ -274,7 +282,8 @@ def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
 
     Returns (out, h). out: bf16, or an Fp8Tensor for out_dtype
     torch.float8_e4m3fn. h: written to `residual_out` where that is given (x
-    itself for an update in place), else to a new tensor; x itself without y.
+    itself for an update in place, or a tensor apart from x and y), else to a
+    new tensor; x itself without y.
     """
     _check_cuda("x", x, (torch.float32, torch.bfloat16), 2)
     if x.dim() > 3:
@@ -297,13 +306,20 @@ def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
         if y.shape != x.shape or y.device != x.device:
             raise ValueError(f"y {tuple(y.shape)} must have x's shape {tuple(x.shape)} and device")
     total = x
-    if y is not None:
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None \
-            else residual_out
+    if y is not None and residual_out is None:
+        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif y is not None:
+        total = residual_out
         if total.shape != x.shape or total.dtype != x.dtype or total.device != x.device:
             raise ValueError("residual_out must have x's shape, type and device")
         if _row_stride(total) is None:
             raise ValueError("residual_out must have evenly spaced rows of contiguous features")
+        if total is not x and total.numel():
+            t0, t1 = _span(total)
+            for other in (x, y):
+                o0, o1 = _span(other)
+                if t0 < o1 and o0 < t1 and not (other is x and t0 == o0 and total.stride() == x.stride()):
+                    raise ValueError("residual_out must be x or lie apart from x and y")
         if total.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("residual_out requires a gradient: this operator is inference only")
     dev = x.device
