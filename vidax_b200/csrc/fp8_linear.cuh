@@ -19,7 +19,7 @@
 // barrier phases run on across tiles, so the next tile's loads and products
 // start while the last one is rounded and stored. A finished tile leaves
 // through shared memory by TMA (full 128-byte lines, edges clipped by the
-// tensor map); an output that TMA cannot address is stored element by element.
+// tensor map); an output that TMA cannot address leaves it row by row.
 //
 // What bounds it, measured on 9472 x 8960 -> 2048 (177-184 us, 1930 TFLOP/s, a
 // plain e4m3 product of the library 131 us): the power cap (1000 W, at 1425 of
@@ -36,6 +36,8 @@
 // gives up soon: all roles still walk all of their blocks, so that nothing
 // waits for an arrival that does not come, and the output is not valid.
 #pragma once
+
+#include <type_traits>
 
 #include "fp8_common.cuh"
 
@@ -513,39 +515,41 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           p.out_scale[row * p.os_rs + static_cast<long long>(col / kBlock) * p.os_bs] = s;
       }
       constexpr int kElem = kOut == kOutBf16 ? 2 : kOut == kOutFloat ? 4 : 1;
-      if (p.tma_out) {
-        // 32 rows x kWide bytes at a time, 16-byte pieces swizzled as the
-        // tensor map says, so that lanes (rows) hit different banks
-        constexpr int kWide = kCols * kElem < 128 ? kCols * kElem : 128;
-        constexpr int kWideCols = kWide / kElem;
-        const uint32_t buf = sbase + Dm::kStore + warp * 4096;
-        const uint32_t mine = buf + lane * kWide;
-        const uint32_t swz = kWide == 128 ? (lane & 7) : kWide == 64 ? ((lane >> 1) & 3) : 0;
+      // 32 rows x kWide bytes at a time, 16-byte pieces swizzled as the tensor
+      // map says, so that lanes (rows) hit different banks
+      constexpr int kWide = kCols * kElem < 128 ? kCols * kElem : 128;
+      constexpr int kWideCols = kWide / kElem;
+      uint8_t* const buf = smem + Dm::kStore + warp * 4096;
+      const uint32_t mine = smem_u32(buf) + lane * kWide;
+      auto swizzle = [](int r) { return kWide == 128 ? r & 7 : kWide == 64 ? (r >> 1) & 3 : 0; };
 #pragma unroll
-        for (int c = 0; c < kCols; c += kWideCols) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
+      for (int c = 0; c < kCols; c += kWideCols) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < kWide / 16; ++i) {
-            uint32_t q[4];
-            lin_pack16<kOut>(acc + c + i * (16 / kElem), inv, q);
-            st_shared_v4(mine + ((i ^ swz) << 4), q[0], q[1], q[2], q[3]);
-          }
+        for (int i = 0; i < kWide / 16; ++i) {
+          uint32_t q[4];
+          lin_pack16<kOut>(acc + c + i * (16 / kElem), inv, q);
+          st_shared_v4(mine + ((i ^ swizzle(lane)) << 4), q[0], q[1], q[2], q[3]);
+        }
+        if (p.tma_out) {
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && c < have && row < p.m) lin_store(&tm_o, buf, col + c, row);
-        }
-      } else if (live) {
+          if (lane == 0 && c < have && row < p.m) lin_store(&tm_o, smem_u32(buf), col + c, row);
+        } else {  // rows off the 16-byte boundaries: neighbours by neighbouring lanes
+          __syncwarp();
+          const int rows = min(32, p.m - (row - lane)), cols = min(kWideCols, have - c);
+          using Word = std::conditional_t<kElem == 4, uint32_t,
+                                          std::conditional_t<kElem == 2, uint16_t, uint8_t>>;
+          Word* out = static_cast<Word*>(p.out) + (row - lane) * p.out_stride + col + c;
+          for (int r = 0; r < rows; ++r, out += p.out_stride) {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          if (j < have) {
-            const long long at = row * p.out_stride + col + j;
-            if constexpr (kOut == kOutBf16)
-              static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(acc[j]);
-            else if constexpr (kOut == kOutFloat) static_cast<float*>(p.out)[at] = acc[j];
-            else
-              static_cast<uint8_t*>(p.out)[at] =
-                  static_cast<uint8_t>(pack_e4m3x4(acc[j] * inv, 0.f, 0.f, 0.f));
+            for (int e = lane; e < kWideCols; e += 32) {
+              const int at = e * kElem;
+              if (e < cols)
+                out[e] = *reinterpret_cast<const Word*>(buf + r * kWide +
+                                                        (((at >> 4) ^ swizzle(r)) << 4) + (at & 15));
+            }
           }
         }
       }

@@ -12,15 +12,17 @@
 // two MMAs. The warps' sums meet in shared memory and are added in the order
 // of the warps: the result does not depend on timing.
 //
-// One token, weights from HBM, in us (floor by bytes / this / the 128-row
-// tiles): 1536 -> 1536 0.4 / 2.5 / 5.5, 1536 -> 9216 2.2 / 5.7 / 8.9,
-// 8960 -> 1536 2.1 / 6.2 / 17.5, 5120 -> 13824 11 / 17 / 28. From nine rows on
-// the second MMA per load shows (1536 -> 9216: 9.6, the tiles 8.5), and only
-// where few CTAs share many features is this form still ahead (8960 -> 1536:
-// 9.1 against 17.5).
+// Eight tokens, weights from HBM, in us (floor by bytes / this / the better of
+// the 128-row tiles): 1536 -> 1536 0.4 / 2.6 / 5.5, 1536 -> 9216 2.2 / 6.1 /
+// 9.0, 8960 -> 1536 2.1 / 6.9 / 17.3, 5120 -> 13824 11 / 17 / 25. Sixteen: 3.0 /
+// 5.6, 6.7 / 8.8, 8.6 / 17.2 and 20 / 24; 13824 -> 5120 is even at 25. Beyond,
+// the MMAs per load show.
 //
 // The e4m3 output needs the largest magnitude of 128 features: the eight CTAs
 // that hold them form a cluster and read it from one another's shared memory.
+// That costs some 3 us (1536 -> 8960 with GELU: one token 8.0 against 9.7 with
+// the tiles, sixteen 12.2 against 9.4, so past eight tokens the tiles take
+// outputs with many CTAs; 8960 -> 1536 stays ahead, 8.6 against 22.6).
 #pragma once
 
 #include <type_traits>
@@ -69,7 +71,7 @@ __device__ __forceinline__ uint4 few_load(const uint8_t* row, int k0, int k) {
 }
 
 template <int kWarps, int kNT, int kOut>
-__global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
+__global__ void __launch_bounds__(kWarps * 32, (kNT == 1 ? 24 : 16) / kWarps)
     linear_few_kernel(const __grid_constant__ FewParams p) {
   constexpr int kTok = 8 * kNT;
   __shared__ float part[kWarps][kTok][kFewCols + 1];
@@ -136,8 +138,10 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
   };
   const int full = p.k / kBlock;
   int kb = warp;
-  for (; kb + 3 * kWarps < full; kb += 4 * kWarps)
-    blocks(kb, std::integral_constant<int, 4>(), std::false_type());
+  if constexpr (kNT == 1) {  // (16 tokens' operands of four blocks do not fit the registers)
+    for (; kb + 3 * kWarps < full; kb += 4 * kWarps)
+      blocks(kb, std::integral_constant<int, 4>(), std::false_type());
+  }
   for (; kb + kWarps < full; kb += 2 * kWarps)
     blocks(kb, std::integral_constant<int, 2>(), std::false_type());
   for (; kb < full; kb += kWarps) blocks(kb, std::integral_constant<int, 1>(), std::false_type());

@@ -397,7 +397,8 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   if (a->variant == 0)  // (measured: fp8_linear_few.cuh)
-    few = a->m <= 8 || (a->m <= kFewMost && few_wide(a->n, p.kblocks, sms));
+    few = a->m <= kFewMost &&
+          (out_idx != kOutE4m3 || a->m <= 8 || few_wide(a->n, p.kblocks, sms));
   if (few) {
     FewParams f{static_cast<const uint8_t*>(a->x), static_cast<const uint8_t*>(a->w),
                 static_cast<long long>(xst), static_cast<long long>(wst), a->k, p};
