@@ -509,6 +509,40 @@ def test_linear_cold_operands(variant, m, n, k):
     assert bool(torch.stack(same).all())
 
 
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: their last rows equal the same rows
+    computed alone."""
+    import vidax_b200 as vx
+    rows, dim = 170000, 13000
+    x = torch.empty((rows, dim), dtype=torch.bfloat16, device="cuda")
+    x.normal_(generator=_gen(70))
+    q = vx.quantize_fp8(x)
+    ref = vx.quantize_fp8(x[-9:].clone())
+    assert torch.equal(q.data[-9:].float(), ref.data.float()) and torch.equal(q.scale[-9:], ref.scale)
+    del q
+    gate = torch.full((1, dim), 0.5, device="cuda")
+    o, total = vx.add_norm(x, x, gate, out_dtype=torch.float8_e4m3fn)
+    oref, tref = vx.add_norm(x[-9:].clone(), x[-9:].clone(), gate, out_dtype=torch.float8_e4m3fn)
+    assert torch.equal(o.data[-9:].float(), oref.data.float()) and torch.equal(o.scale[-9:], oref.scale)
+    assert torch.equal(total[-9:], tref)
+    del x, o, total
+    m, k = 260000, 130
+    g = _gen(71)
+    a = vx.quantize_fp8(torch.randn((m, k), generator=g, device="cuda"))
+    tail = vx.Fp8Tensor(a.data[-200:], a.scale[-200:])
+    for n, out in ((8704, torch.bfloat16), (8703, torch.bfloat16), (8703, torch.float8_e4m3fn)):
+        w = vx.quantize_fp8(torch.randn((n, k), generator=g, device="cuda"), 128)
+        y = vx.linear_fp8(a, w, out_dtype=out)
+        ref = vx.linear_fp8(tail, w, out_dtype=out)
+        _ok()
+        if out == torch.bfloat16:
+            assert torch.equal(y[-200:], ref)
+        else:
+            assert torch.equal(y.data[-200:].float(), ref.data.float())
+            assert torch.equal(y.scale[-200:], ref.scale)
+        del y, ref
+
+
 # ------------------------------------------------------------------ together
 
 

@@ -296,116 +296,116 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp >= kFeed) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Dm::kFeedRegs));
-  if (warp == kFeed) {
-    // ------------------------------------------------------------ producer
-    const uint64_t policy = l2_policy_evict_last();
-    const bool issuer = elect_one();
-    Ring<S> st;
-    for (int t = unit0; t < p.tiles; t += unit_step) {
-      int tm, tn;
-      lin_tile(p, t, tm, tn);
-      const int row = tm * kLinRows, col = tn * kBN;
-      for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
-        mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
-        const uint32_t dst = sbase + st.i * Dm::kStageBytes;
-        if (issuer) {
-          mbar_expect_tx(bar(kLinFull + st.i), Dm::kStageBytes);
-          lin_load(dst, &tm_x, bar(kLinFull + st.i), kb * kBlock, row, policy);
-          lin_load(dst + Dm::kABytes, &tm_w, bar(kLinFull + st.i), kb * kBlock, col, policy);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Dm::kFeedRegs));
+    if (warp == kFeed) {
+      // ------------------------------------------------------------ producer
+      const uint64_t policy = l2_policy_evict_last();
+      const bool issuer = elect_one();
+      Ring<S> st;
+      for (int t = unit0; t < p.tiles; t += unit_step) {
+        int tm, tn;
+        lin_tile(p, t, tm, tn);
+        const int row = tm * kLinRows, col = tn * kBN;
+        for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
+          mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
+          const uint32_t dst = sbase + st.i * Dm::kStageBytes;
+          if (issuer) {
+            mbar_expect_tx(bar(kLinFull + st.i), Dm::kStageBytes);
+            lin_load(dst, &tm_x, bar(kLinFull + st.i), kb * kBlock, row, policy);
+            lin_load(dst + Dm::kABytes, &tm_w, bar(kLinFull + st.i), kb * kBlock, col, policy);
+          }
         }
       }
-    }
-    if (*abort_flag) {
-      // the loads in flight land before the CTA gives its memory back
+      if (*abort_flag) {
+        // the loads in flight land before the CTA gives its memory back
+        const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
+        const long long steps = static_cast<long long>(tiles) * p.kblocks;
+        for (int i = 0; i < S && i < steps; ++i) {
+          st.i = st.i == 0 ? S - 1 : st.i - 1;
+          if (st.i == S - 1) st.phase ^= 1u;
+          mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
+        }
+      }
+    } else if (warp == kFeed + 1 || warp == kFeed + 3) {
+      // ------------------------------------------------------------ MMA issuers
+      // Two warps take the blocks in turn, so that one's waits and issues overlap
+      // the other's. Blocks are independent (each starts a product), so tiles do
+      // not matter here. The whole warp walks the loop and one lane issues:
+      // addresses and descriptors then stay in uniform registers.
+      constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows, kBN);
+      const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
+      const bool issuer = elect_one();
+      const int first = warp == kFeed + 3 ? 1 : 0;
       const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
       const long long steps = static_cast<long long>(tiles) * p.kblocks;
-      for (int i = 0; i < S && i < steps; ++i) {
-        st.i = st.i == 0 ? S - 1 : st.i - 1;
-        if (st.i == S - 1) st.phase ^= 1u;
-        mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
+      Ring<S> st;
+      Ring<kBufs> ac;
+      if (first) {
+        st.next();
+        ac.next();
       }
-    }
-  } else if (warp == kFeed + 1 || warp == kFeed + 3) {
-    // ------------------------------------------------------------ MMA issuers
-    // Two warps take the blocks in turn, so that one's waits and issues overlap
-    // the other's. Blocks are independent (each starts a product), so tiles do
-    // not matter here. The whole warp walks the loop and one lane issues:
-    // addresses and descriptors then stay in uniform registers.
-    constexpr uint32_t kIdesc = idesc_e4m3_f32(kLinRows, kBN);
-    const uint64_t desc0 = sdesc_sw128(sbase, 16, 1024);
-    const bool issuer = elect_one();
-    const int first = warp == kFeed + 3 ? 1 : 0;
-    const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
-    const long long steps = static_cast<long long>(tiles) * p.kblocks;
-    Ring<S> st;
-    Ring<kBufs> ac;
-    if (first) {
-      st.next();
-      ac.next();
-    }
-    // steps, and then once more for each buffer, so that every arrival of the
-    // sums at the named barriers is met
-    for (long long i = first; i < steps + kBufs; i += 2) {
-      if (i >= kBufs && i - kBufs < steps)  // the product before in this buffer has been read
-        lin_buffer_sync<Dm::kSumWG * 128 + 32>(ac.i);
-      if (i < steps) {
-        // Only after that: an issuer sees every other block, and with an odd
-        // number of stages the stage's last round was the other issuer's. A
-        // wait tells odd rounds from even ones only, so a look while that
-        // round's load (block i - kStages) is under way would pass. Once block
-        // i - kBufs has been added, so has the one before it in this stage
-        // (kBufs < kStages).
-        mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
-        tc_fence_after();
-        const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
-        const uint64_t db = da + (Dm::kABytes >> 4);
-        const uint32_t acc = tmem + ac.i * kBN;
-        if (issuer) {
+      // steps, and then once more for each buffer, so that every arrival of the
+      // sums at the named barriers is met
+      for (long long i = first; i < steps + kBufs; i += 2) {
+        if (i >= kBufs && i - kBufs < steps)  // the product before in this buffer has been read
+          lin_buffer_sync<Dm::kSumWG * 128 + 32>(ac.i);
+        if (i < steps) {
+          // Only after that: an issuer sees every other block, and with an odd
+          // number of stages the stage's last round was the other issuer's. A
+          // wait tells odd rounds from even ones only, so a look while that
+          // round's load (block i - kStages) is under way would pass. Once block
+          // i - kBufs has been added, so has the one before it in this stage
+          // (kBufs < kStages).
+          mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
+          tc_fence_after();
+          const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
+          const uint64_t db = da + (Dm::kABytes >> 4);
+          const uint32_t acc = tmem + ac.i * kBN;
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
-            lin_mma(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
-          tc_commit(bar(kLinDone + st.i));
+            for (int kk = 0; kk < 4; ++kk)  // 32 features per MMA
+              lin_mma(acc, da + 2 * kk, db + 2 * kk, kIdesc, kk > 0 ? 1u : 0u);
+            tc_commit(bar(kLinDone + st.i));
+          }
+        }
+        __syncwarp();  // the named barrier wants the warp together
+        st.next();
+        st.next();
+        ac.next();
+        ac.next();
+      }
+      if (*abort_flag && issuer) {
+        tc_commit(bar(kLinDrain + first));
+        mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
+      }
+    } else if (warp == kFeed + 2) {
+      // ------------------------------------------------------------ scales
+      Ring<kScaleGroups> sg;
+      for (int t = unit0; t < p.tiles; t += unit_step) {
+        int tm, tn;
+        lin_tile(p, t, tm, tn);
+        const int row = tm * kLinRows + lane;
+        const int col = tn * kBN + (lane & (Dm::kSumWG - 1)) * kCols;
+        const float* xs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
+        const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
+        for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
+          mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
+          const int n = min(kGroupBlocks, p.kblocks - kb0);
+          uint32_t dst = sbase + Dm::kScales + sg.i * (kGroupBlocks * kScaleFloats * 4) + lane * 4;
+          for (int kb = kb0; kb < kb0 + n; ++kb, dst += kScaleFloats * 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
+            if (lane < Dm::kSumWG) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
+          }
+          cp_async_arrive(bar(kLinScaleFull + sg.i));
         }
       }
-      __syncwarp();  // the named barrier wants the warp together
-      st.next();
-      st.next();
-      ac.next();
-      ac.next();
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    if (*abort_flag && issuer) {
-      tc_commit(bar(kLinDrain + first));
-      mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
-    }
-  } else if (warp == kFeed + 2) {
-    // ------------------------------------------------------------ scales
-    Ring<kScaleGroups> sg;
-    for (int t = unit0; t < p.tiles; t += unit_step) {
-      int tm, tn;
-      lin_tile(p, t, tm, tn);
-      const int row = tm * kLinRows + lane;
-      const int col = tn * kBN + (lane & (Dm::kSumWG - 1)) * kCols;
-      const float* xs[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
-      const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
-      for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
-        mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
-        const int n = min(kGroupBlocks, p.kblocks - kb0);
-        uint32_t dst = sbase + Dm::kScales + sg.i * (kGroupBlocks * kScaleFloats * 4) + lane * 4;
-        for (int kb = kb0; kb < kb0 + n; ++kb, dst += kScaleFloats * 4) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            cp_async4(dst + 128 * i, xs[i] + kb * p.xs_bs, row + 32 * i < p.m);
-          if (lane < Dm::kSumWG) cp_async4(dst + 512, ws + kb * p.ws_bs, col < p.n);
-        }
-        cp_async_arrive(bar(kLinScaleFull + sg.i));
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Dm::kSumRegs));
     // ------------------------------------------------------------ sums and output

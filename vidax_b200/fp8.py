@@ -13,7 +13,11 @@ features (`Fp8Tensor`), and three kernels make and use it:
                      tanh GELU, its output in bf16, float32 or e4m3 again.
 
 `vidax_b200.wan_dit.quantize_params` gives a whole DiT's weights this form.
-Inference only, like the rest of this package: the outputs carry no gradient.
+Inference only, like the rest of this package: inputs that require a gradient
+are refused while gradients are recorded. The operators keep nothing between
+calls (no workspace), so any number of them may run at once and in captured
+graphs; as with the other kernels, the first call on a device comes before a
+capture.
 """
 from __future__ import annotations
 
