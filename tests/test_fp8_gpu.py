@@ -206,6 +206,20 @@ def test_add_norm(b, l, dim, norm, stream, out):
     _check_norm(c, norm, o, total)
 
 
+@pytest.mark.parametrize("out", ["fp8", "bf16"])
+@pytest.mark.parametrize("stream", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [129, 515, 1187, 1500, 2047, 2500])
+def test_add_norm_odd_widths_many_rows(dim, stream, out):
+    """Rows off the 16-byte boundaries, enough of them for the variants with
+    few warps per row."""
+    import vidax_b200 as vx
+    c = _norm_case(1, 700, dim, stream, dim)
+    o, total = vx.add_norm(**c, norm="layer",
+                           out_dtype=torch.float8_e4m3fn if out == "fp8" else torch.bfloat16)
+    _ok()
+    _check_norm(c, "layer", o, total)
+
+
 @pytest.mark.parametrize("missing", ["y", "gate", "weight", "bias", "scale", "shift", "all"])
 def test_add_norm_optional_parts(missing):
     import vidax_b200 as vx

@@ -105,6 +105,14 @@ __device__ __forceinline__ void put4(uint32_t* w, const uint4& v) {
   w[2] = v.z;
   w[3] = v.w;
 }
+// 0 for the elements past the first `have`.
+__device__ __forceinline__ void cut8(float (&f)[8], int have) {
+  if (have < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i >= have) f[i] = 0.f;
+  }
+}
 // The 16-byte piece `k` after the one that holds `p`, if bytes [16 k, ...) of
 // it are wanted (`bytes` from p on).
 __device__ __forceinline__ uint4 piece(const void* p, int k, int bytes) {
@@ -135,7 +143,8 @@ struct Raw<float, false> {
     put4(w + 8, c);
     shift_words(w, q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < have ? __uint_as_float(w[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+    cut8(f, have);
   }
 };
 template <>
@@ -159,9 +168,10 @@ struct Raw<__nv_bfloat16, false> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = __funnelshift_r(w[i], w[i + 1], (at & 2u) * 8u);
-      f[2 * i] = 2 * i < have ? __uint_as_float(v << 16) : 0.f;
-      f[2 * i + 1] = 2 * i + 1 < have ? __uint_as_float(v & 0xffff0000u) : 0.f;
+      f[2 * i] = __uint_as_float(v << 16);
+      f[2 * i + 1] = __uint_as_float(v & 0xffff0000u);
     }
+    cut8(f, have);
   }
 };
 
