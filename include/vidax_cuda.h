@@ -480,6 +480,17 @@ typedef struct vx_linear_fp8_args {
 } vx_linear_fp8_args;
 int vx_linear_fp8(const vx_linear_fp8_args* args, vx_stream_t stream);
 
+/* Self-test of vx_linear_fp8's waits (failure detection without a GPU fault):
+ * the same product in the same kernel, in which one role falls silent at its
+ * block `after` (0: none; 1: loads, 2: scales, 3: an adding warp's signals),
+ * so that the others' waits run out of `limit_cycles` SM
+ * cycles. The call returns as ever; the kernel ends with a timeout code in the
+ * status word (vx_device_status) and an output that is not valid, and the
+ * context stays usable. e4m3 outputs take the 256-column tile, bf16 ones the
+ * 64-column tile. */
+int vx_selftest_linear_fp8(const vx_linear_fp8_args* args, int32_t role, int32_t after,
+                           int64_t limit_cycles, vx_stream_t stream);
+
 /* Self-test of the bounded-wait machinery (failure detection without a GPU
  * fault): runs one CTA that waits on an mbarrier nothing arrives on, through
  * the same bounded wait the kernels use, with a limit of `limit_cycles` SM

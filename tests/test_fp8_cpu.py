@@ -168,3 +168,16 @@ def test_c_null_and_empty_calls():
     assert _rc("vx_quantize_fp8", _args(fp8.QuantizeFp8Args, **{**QOK, "rows": 0}))[0] == 0
     assert _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, "rows": 0}))[0] == 0
     assert _rc("vx_linear_fp8", _args(fp8.LinearFp8Args, **{**LOK, "m": 0}))[0] == 0
+
+
+@pytest.mark.parametrize("change,call,code", [
+    ({}, (-1, 0, 1000), 1), ({}, (4, 0, 1000), 1), ({}, (1, -1, 1000), 1), ({}, (1, 0, 0), 1),
+    ({}, (1, 0, 1 << 33), 1), (dict(variant=1), (1, 0, 1000), 2), (dict(out_type=0), (1, 0, 1000), 2),
+    (dict(m=-1), (1, 0, 1000), 1), (dict(x=None), (1, 0, 1000), 1)])
+def test_linear_selftest_refusals(change, call, code):
+    from vidax_b200 import _lib, fp8
+    fn = _lib.load().vx_selftest_linear_fp8
+    a = _args(fp8.LinearFp8Args, **{**LOK, **change})
+    role, after, limit = call
+    assert fn(ctypes.byref(a), role, after, ctypes.c_int64(limit), None) == code
+    assert fn(None, 1, 0, ctypes.c_int64(1000), None) == 1

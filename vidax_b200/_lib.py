@@ -39,6 +39,7 @@ EXPORTED_SYMBOLS = (
     "vx_quantize_fp8",
     "vx_add_norm",
     "vx_linear_fp8",
+    "vx_selftest_linear_fp8",
     "vx_memcpy_rows_async",
     "vx_selftest_wait_timeout",
     "vx_comm_get_unique_id",

@@ -32,9 +32,12 @@
 // 2 %; two CTAs per SM with half of TMEM each, or two sets of warpgroups on
 // tiles in turn, were 25 to 60 % slower.
 //
-// If a wait runs out of its limit, the abort flag is up and every later wait
-// gives up soon: all roles still walk all of their blocks, so that nothing
-// waits for an arrival that does not come, and the output is not valid.
+// If a wait runs out of its limit, it raises the abort flag, and with the flag
+// up the other waits for loads, scales and row maxima give up soon. The loads
+// stop there; the issuers and the adding warps still walk all of their blocks,
+// in step with one another (lin_wait_product says why that always ends). Then
+// the loads in flight are waited for (with a limit), and the CTA ends with the
+// code in the status word and an output that is not valid.
 #pragma once
 
 #include <type_traits>
@@ -62,7 +65,12 @@ struct LinearParams {
   int act;
   int tma_out;                  // the output goes through tm_o
   int* status;
+  // the self-test's form only: the wait limit, and the role (LinDrop) that
+  // falls silent at its block `drop_at`
+  long long limit;
+  int drop, drop_at;
 };
+enum LinDrop : int { kDropNone = 0, kDropLoads, kDropScales, kDropSums, kNumDrops };
 
 constexpr int kLinRows = 128;          // activation rows per CTA
 constexpr int kGroupM = 8;             // row tiles that share a pass over the weights
@@ -107,12 +115,12 @@ struct LinDims {
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
 };
 
-// control block: barriers, then the TMEM address and the abort flag
+// control block: barriers, then the TMEM address, the abort flag and the
+// number of blocks loaded
 enum : int {
   kLinFull = 0,        // stages: operands landed
   kLinDone = 8,        // stages: their MMAs are done (the stage is free, the product complete)
   kLinAmax = 24,       // every warpgroup's largest magnitudes are written
-  kLinDrain = 26,      // 2: an issuer's MMAs are done (after an abort)
   kLinScaleFull = 28,  // 4: a group's scales landed
   kLinScaleEmpty = 32, // 4: read by every adding warp
   kLinBars = 36,
@@ -224,8 +232,9 @@ __device__ __forceinline__ void lin_pack16(const float* v, float inv, uint32_t (
 
 // Hand-over of a TMEM buffer from the sums to an MMA issuer over a named
 // barrier: a look at one in shared memory takes 110 cycles while the tensor
-// core reads its operands. It needs no time limit of its own: every adding
-// warp gets to every block, at the latest when its waits have given up.
+// core reads its operands (9472 x 8960 -> 2048: 196 us with an mbarrier, 171
+// so; 4680 x 1536 -> 4608: 47.6 and 44.6). A named barrier counts arrivals, not
+// who arrived, and has no limit; see lin_wait_product.
 template <int kThreads>
 __device__ __forceinline__ void lin_buffer_arrive(int buf) {
   asm volatile("bar.arrive %0, %1;" ::"r"(buf + 1), "n"(kThreads) : "memory");
@@ -233,6 +242,33 @@ __device__ __forceinline__ void lin_buffer_arrive(int buf) {
 template <int kThreads>
 __device__ __forceinline__ void lin_buffer_sync(int buf) {
   asm volatile("bar.sync %0, %1;" ::"r"(buf + 1), "n"(kThreads) : "memory");
+}
+
+// An adding warp's wait for a block's product. It does not give up with the
+// abort flag, because the warp arrives for the block at a named barrier next:
+// a warp that ran ahead would arrive twice in one generation, and an issuer
+// later wait for an arrival that nobody has left to make. It needs not to. An
+// issuer commits for every block, whether its wait for the load was met or gave
+// up, after it has taken the hand-over of the block kBufs before in the same
+// buffer. So, by induction over the blocks, every product's barrier completes
+// and every hand-over comes: block i's product needs the hand-over of block
+// i - kBufs, waits that give up and the MMAs' own completion (before which a
+// CTA could not end anyway, since they read its memory); the hand-over of block
+// i needs every adding warp to have seen product i and waits that give up. And
+// an arrival made after product i is seen is one for that block's generation.
+// The first wait to run out takes one limit, after which the flag is up; four
+// is longer than any of this can take.
+__device__ __forceinline__ void lin_wait_product(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                 int* status, long long limit) {
+  if (mbar_try_wait(bar, parity)) return;
+  const long long t0 = clock64();
+  for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+    if ((it & 255u) == 0u && clock64() - t0 > 4 * limit) {
+      *abort_flag = 1;
+      atomicOr(status, kDevTimeoutSoftmax);
+      return;
+    }
+  }
 }
 
 // Output tile -> (row tile, column tile): kGroupM row tiles run down before
@@ -247,7 +283,8 @@ __device__ __forceinline__ void lin_tile(const LinearParams& p, int t, int& tm, 
   tm = g * kGroupM + (r - tn * gm);
 }
 
-template <int kBN, int kOut>
+// kTest: the form of the self-test (a role falls silent, short wait limit).
+template <int kBN, int kOut, bool kTest = false>
 __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ LinearParams p) {
@@ -262,6 +299,8 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
   auto bar = [&](int i) -> uint32_t { return sbase + Dm::kCtl + 8u * i; };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Dm::kCtl + 8 * kLinBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Dm::kCtl + 8 * kLinBars + 4);
+  volatile long long* loaded = reinterpret_cast<volatile long long*>(smem + Dm::kCtl + 8 * kLinBars + 8);
+  const long long limit = kTest ? p.limit : kWaitLimitCycles;
   // The shuffle tells the compiler that the warp index is the same in all lanes.
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -277,9 +316,8 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
       mbar_init(bar(kLinScaleEmpty + i), kFeed);
     }
     mbar_init(bar(kLinAmax), 32 * kFeed);
-    mbar_init(bar(kLinDrain), 1);
-    mbar_init(bar(kLinDrain + 1), 1);
     *abort_flag = 0;
+    *loaded = 0;
     fence_barrier_init();
   }
   if (warp == kFeed + 1) {
@@ -302,12 +340,22 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
       const uint64_t policy = l2_policy_evict_last();
       const bool issuer = elect_one();
       Ring<S> st;
-      for (int t = unit0; t < p.tiles; t += unit_step) {
+      long long n = 0;  // blocks loaded
+      bool ok = true;
+      for (int t = unit0; t < p.tiles && ok; t += unit_step) {
         int tm, tn;
         lin_tile(p, t, tm, tn);
         const int row = tm * kLinRows, col = tn * kBN;
         for (int kb = 0; kb < p.kblocks; ++kb, st.next()) {
-          mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
+          ok = mbar_wait(bar(kLinDone + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad, limit);
+          // After an abort a stage's MMAs may be done without its load: the
+          // barrier is armed again only when the load before has landed.
+          ok = ok && mbar_wait(bar(kLinFull + st.i), st.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad,
+                               limit);
+          if (kTest && p.drop == kDropLoads && n >= p.drop_at) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          ++n;
           const uint32_t dst = sbase + st.i * Dm::kStageBytes;
           if (issuer) {
             mbar_expect_tx(bar(kLinFull + st.i), Dm::kStageBytes);
@@ -316,16 +364,7 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           }
         }
       }
-      if (*abort_flag) {
-        // the loads in flight land before the CTA gives its memory back
-        const int tiles = unit0 < p.tiles ? (p.tiles - 1 - unit0) / unit_step + 1 : 0;
-        const long long steps = static_cast<long long>(tiles) * p.kblocks;
-        for (int i = 0; i < S && i < steps; ++i) {
-          st.i = st.i == 0 ? S - 1 : st.i - 1;
-          if (st.i == S - 1) st.phase ^= 1u;
-          mbar_wait_drain(bar(kLinFull + st.i), st.phase, p.status);
-        }
-      }
+      if (lane == 0) *loaded = n;
     } else if (warp == kFeed + 1 || warp == kFeed + 3) {
       // ------------------------------------------------------------ MMA issuers
       // Two warps take the blocks in turn, so that one's waits and issues overlap
@@ -356,7 +395,7 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           // round's load (block i - kStages) is under way would pass. Once block
           // i - kBufs has been added, so has the one before it in this stage
           // (kBufs < kStages).
-          mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma);
+          mbar_wait(bar(kLinFull + st.i), st.phase, abort_flag, p.status, kDevTimeoutMma, limit);
           tc_fence_after();
           const uint64_t da = desc0 + static_cast<uint32_t>(st.i * (Dm::kStageBytes >> 4));
           const uint64_t db = da + (Dm::kABytes >> 4);
@@ -374,10 +413,6 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
         ac.next();
         ac.next();
       }
-      if (*abort_flag && issuer) {
-        tc_commit(bar(kLinDrain + first));
-        mbar_wait_drain(bar(kLinDrain + first), 0, p.status);
-      }
     } else if (warp == kFeed + 2) {
       // ------------------------------------------------------------ scales
       Ring<kScaleGroups> sg;
@@ -392,7 +427,11 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           xs[i] = p.xs + (row + 32 * i < p.m ? (row + 32 * i) * p.xs_rs : 0);
         const float* ws = p.ws + (col < p.n ? static_cast<long long>(col / kBlock) * p.ws_rs : 0);
         for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
-          mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad);
+          if (kTest && p.drop == kDropScales && kb0 >= p.drop_at) {
+            t = p.tiles;  // no more tiles either
+            break;
+          }
+          mbar_wait(bar(kLinScaleEmpty + sg.i), sg.phase ^ 1u, abort_flag, p.status, kDevTimeoutLoad, limit);
           const int n = min(kGroupBlocks, p.kblocks - kb0);
           uint32_t dst = sbase + Dm::kScales + sg.i * (kGroupBlocks * kScaleFloats * 4) + lane * 4;
           for (int kb = kb0; kb < kb0 + n; ++kb, dst += kScaleFloats * 4) {
@@ -455,18 +494,19 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
       }
       fetch_bias(t + unit_step, bias);
       for (int kb0 = 0; kb0 < p.kblocks; kb0 += kGroupBlocks, sg.next()) {
-        mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag, p.status, kDevTimeoutSoftmax);
+        mbar_wait(bar(kLinScaleFull + sg.i), sg.phase, abort_flag, p.status, kDevTimeoutSoftmax, limit);
         const volatile float* sp = scale_s + sg.i * (kGroupBlocks * kScaleFloats);
         float sc[kGroupBlocks];  // (of blocks past the last one: not used)
 #pragma unroll
         for (int g = 0; g < kGroupBlocks; ++g)
           sc[g] = sp[g * kScaleFloats + r_in] * sp[g * kScaleFloats + 128 + wg];
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kLinScaleEmpty + sg.i));
+        const bool silent = kTest && p.drop == kDropSums && warp == 0 && kb0 >= p.drop_at;
+        if (lane == 0 && !silent) mbar_arrive(bar(kLinScaleEmpty + sg.i));
 #pragma unroll
         for (int g = 0; g < kGroupBlocks; ++g) {
           if (kb0 + g >= p.kblocks) break;
-          mbar_wait(bar(kLinDone + st.i), st.phase, abort_flag, p.status, kDevTimeoutSoftmax);
+          lin_wait_product(bar(kLinDone + st.i), st.phase, abort_flag, p.status, limit);
           __syncwarp();
           tc_fence_after();
           const uint32_t tm_acc = t_lane + ac.i * kBN;
@@ -506,8 +546,9 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           // next tile's barrier, which every reader of this one has passed.
           volatile float* mine = amax_s + tile_parity * (128 * Dm::kSumWG);
           mine[wg * 128 + r_in] = am;
-          mbar_arrive(bar(kLinAmax));
-          mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status, kDevTimeoutSoftmax);
+          const bool silent = kTest && p.drop == kDropSums && warp == 0 && p.kblocks > p.drop_at;
+          if (!silent) mbar_arrive(bar(kLinAmax));
+          mbar_wait(bar(kLinAmax), tile_parity, abort_flag, p.status, kDevTimeoutSoftmax, limit);
           am = fmaxf(am, mine[(wg ^ 1) * 128 + r_in]);
         }
         const float s = block_scale(am, inv);
@@ -558,9 +599,14 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();  // every role has left; all products have been seen
   tc_fence_after();
   if (warp == kFeed + 1) tmem_dealloc(tmem, 512);
+  if (warp == kFeed && *abort_flag) {  // the stages' last loads land before the memory goes
+    const long long n = *loaded;
+    for (long long i = n > S ? n - S : 0; i < n; ++i)
+      mbar_wait_drain(bar(kLinFull + static_cast<int>(i % S)), static_cast<uint32_t>(i / S) & 1u, p.status);
+  }
 }
 
 }  // namespace fp8

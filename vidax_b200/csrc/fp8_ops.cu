@@ -347,7 +347,16 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
   return launched("add_norm launch");
 }
 
-extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
+namespace {
+
+// The self-test of the wide kernel's waits: the role that falls silent, at
+// which of its blocks, and the wait limit.
+struct LinTest {
+  int drop, after;
+  long long limit;
+};
+
+int linear_call(const vx_linear_fp8_args* a, const LinTest* test, vx_stream_t stream) {
   if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
   if (a->m < 0 || a->n < 1 || a->k < 1)
     return fail(VX_EINVAL, "bad sizes (m %d, n %d, k %d)", a->m, a->n, a->k);
@@ -401,7 +410,7 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
   // One row needs no stride; the kernels want one that is a multiple of 16.
   const uint64_t xst = a->m > 1 ? a->x_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
   const uint64_t wst = a->n > 1 ? a->w_stride : (static_cast<uint64_t>(a->k) + 15) / 16 * 16;
-  if (a->variant == 0)  // (measured: fp8_linear_few.cuh)
+  if (a->variant == 0 && test == nullptr)  // (measured: fp8_linear_few.cuh)
     few = a->m <= kFewMost &&
           (out_idx != kOutE4m3 || a->m <= 8 || few_wide(a->n, p.kblocks, sms));
   if (few) {
@@ -410,8 +419,19 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
     return launch_few(f, out_idx, sms, reinterpret_cast<cudaStream_t>(stream));
   }
 
-  const LinVariant& v = kVariants[a->variant > 0 ? a->variant - 1 : pick_variant(a, sms)];
+  // (the self-test: four adding warpgroups with two TMEM buffers, row maxima
+  // between warpgroups; or two with four buffers)
+  const LinVariant& v = kVariants[test != nullptr      ? (out_idx == kOutE4m3 ? 0 : kNumVariants - 1)
+                                  : a->variant > 0     ? a->variant - 1
+                                                       : pick_variant(a, sms)];
   const void* fn = v.fn[out_idx];
+  if (test != nullptr) {
+    fn = out_idx == kOutE4m3 ? reinterpret_cast<const void*>(&linear_kernel<256, kOutE4m3, true>)
+                             : reinterpret_cast<const void*>(&linear_kernel<64, kOutBf16, true>);
+    p.limit = test->limit;
+    p.drop = test->drop;
+    p.drop_at = test->after;
+  }
   p.tiles_m = (a->m - 1) / kLinRows + 1;
   p.tiles_n = (a->n - 1) / v.bn + 1;
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
@@ -442,4 +462,23 @@ extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
     return vx_internal_cuda_fail(e, "linear_fp8 launch");
   }
   return VX_OK;
+}
+
+}  // namespace
+
+extern "C" int vx_linear_fp8(const vx_linear_fp8_args* a, vx_stream_t stream) {
+  return linear_call(a, nullptr, stream);
+}
+
+extern "C" int vx_selftest_linear_fp8(const vx_linear_fp8_args* a, int32_t role, int32_t after,
+                                      int64_t limit_cycles, vx_stream_t stream) {
+  if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
+  if (role < 0 || role >= kNumDrops || after < 0)
+    return fail(VX_EINVAL, "role must be in [0, %d) and after >= 0", (int)kNumDrops);
+  if (limit_cycles <= 0 || limit_cycles > 4000000000LL)
+    return fail(VX_EINVAL, "limit_cycles must be in (0, 4e9]");
+  if (a->variant != 0 || (a->out_type != VX_TYPE_E4M3 && a->out_type != VX_TYPE_BF16))
+    return fail(VX_EUNSUPPORTED, "the self-test takes variant 0 and an e4m3 or bf16 output");
+  const LinTest test{role, after, limit_cycles};
+  return linear_call(a, &test, stream);
 }
