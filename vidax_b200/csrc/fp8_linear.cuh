@@ -19,7 +19,10 @@
 // barrier phases run on across tiles, so the next tile's loads and products
 // start while the last one is rounded and stored. A finished tile leaves
 // through shared memory by TMA (full 128-byte lines, edges clipped by the
-// tensor map); an output that TMA cannot address leaves it row by row.
+// tensor map); an output that TMA cannot address leaves it row by row, and so
+// do the last columns of rows that do not end on a 16-byte boundary, where the
+// tensor map clips at the next one and up to 15 bytes behind the row would be
+// written.
 //
 // What bounds it, measured on 9472 x 8960 -> 2048 (177-184 us, 1930 TFLOP/s, a
 // plain e4m3 product of the library 131 us): the power cap (1000 W, at 1425 of
@@ -63,7 +66,8 @@ struct LinearParams {
   int m, n, kblocks;
   int tiles_m, tiles_n, tiles;
   int act;
-  int tma_out;                  // the output goes through tm_o
+  int tma_out;                  // the output goes through tm_o: 1 all of it,
+                                // 2 but the boxes that a row ends in
   int* status;
   // the self-test's form only: the wait limit, and the role (LinDrop) that
   // falls silent at its block `drop_at`
@@ -573,11 +577,11 @@ __global__ void __launch_bounds__(LinDims<kBN>::kThreads, 1)
           lin_pack16<kOut>(acc + c + i * (16 / kElem), inv, q);
           st_shared_v4(mine + ((i ^ swizzle(lane)) << 4), q[0], q[1], q[2], q[3]);
         }
-        if (p.tma_out) {
+        if (p.tma_out == 1 || (p.tma_out == 2 && (c + kWideCols <= have || c >= have))) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && c < have && row < p.m) lin_store(&tm_o, smem_u32(buf), col + c, row);
-        } else {  // rows off the 16-byte boundaries: neighbours by neighbouring lanes
+        } else {  // off the 16-byte boundaries: neighbours by neighbouring lanes
           __syncwarp();
           const int rows = min(32, p.m - (row - lane)), cols = min(kWideCols, have - c);
           using Word = std::conditional_t<kElem == 4, uint32_t,

@@ -439,7 +439,9 @@ int linear_call(const vx_linear_fp8_args* a, const LinTest* test, vx_stream_t st
     return fail(VX_EUNSUPPORTED, "too many output tiles (%lld)", tiles);
   p.tiles = static_cast<int>(tiles);
   const int oe = type_size(a->out_type);
-  p.tma_out = aligned(a->out, 16) && a->out_stride * oe % 16 == 0;
+  p.tma_out = !aligned(a->out, 16) || a->out_stride * oe % 16 != 0 ? 0
+              : static_cast<int64_t>(a->n) * oe % 16 == 0              ? 1
+                                                                       : 2;
   if ((rc = vx_internal_status_word(&p.status)) != VX_OK) return rc;
 
   CUtensorMap tx, tw, to;
