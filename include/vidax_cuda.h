@@ -432,8 +432,11 @@ int vx_quantize_fp8(const vx_quantize_fp8_args* args, vx_stream_t stream);
  *   h = x + float(y) * gate[batch]           (y NULL: h = x, nothing is stored at sum)
  *   n = (h - m) / sqrt(mean((h - m)^2) + eps) * weight + bias,  m = 0 (RMS), mean(h) (layer)
  *   out = n * (1 + scale[batch]) + shift[batch]
- * h is rounded to x's type, stored at `sum` (which may be x) and normalised as
- * stored. gate, weight, bias, scale and shift are each optional (NULL). */
+ * h is rounded to x's type, stored at `sum` and normalised as stored. `sum` is
+ * x itself (the same rows) or lies apart from it, and `sum` and `out` lie apart
+ * from y, the vectors and one another, byte for byte (columns of one wider
+ * buffer may stand side by side); VX_EINVAL otherwise. gate, weight, bias, scale
+ * and shift are each optional (NULL). */
 typedef struct vx_add_norm_args {
   const void* x;        /* (rows, dim) x_type */
   const void* y;        /* (rows, dim) bf16 or NULL */

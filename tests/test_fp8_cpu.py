@@ -181,3 +181,63 @@ def test_linear_selftest_refusals(change, call, code):
     role, after, limit = call
     assert fn(ctypes.byref(a), role, after, ctypes.c_int64(limit), None) == code
     assert fn(None, 1, 0, ctypes.c_int64(1000), None) == 1
+
+
+# add_norm: sum at S, 4 rows of 96 floats (384 bytes), 512 bytes apart
+S = P + (1 << 16)
+IN_PLACE = dict(x=S, sum=S, x_stride=128, sum_stride=128, y=P, y_stride=96, out=P + (1 << 18), out_stride=96)
+
+
+@pytest.mark.parametrize("change", [
+    dict(y=S), dict(y=S + 512, y_stride=256),            # y under the stream, a row further on
+    dict(y=S - 2), dict(y=S - 3 * 192 + 2, y_stride=96), # its last bytes in the first row
+    dict(y=S + 380, y_stride=256),                       # the end of a row, then the gap
+    dict(y=S + 512 - 190, y_stride=256),                 # the gap, then the next row's start
+    dict(sum=S + 512), dict(sum=S - 512), dict(sum=S + 4), dict(sum=S, sum_stride=96),
+    dict(gate=S + 64, gate_stride=0), dict(scale=S + 1000, scale_stride=96),
+    dict(shift=S - 384 - 512, shift_stride=224), dict(weight=S + 3 * 512 + 380), dict(bias=S - 380),
+    dict(out=S), dict(out=S + 100, out_stride=512), dict(out=P + 96, out_type=1),
+    dict(weight=P + (1 << 18) + 4), dict(x_type=1, y=S + 64, y_stride=128)])
+def test_add_norm_c_refuses_overlaps(change):
+    """Written memory that is read for other rows, in place and not: found from
+    the addresses alone, before anything is launched."""
+    from vidax_b200 import fp8
+    rc, msg = _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, **IN_PLACE, **change}))
+    assert rc == 1 and "apart" in msg
+
+
+@pytest.mark.parametrize("change", [
+    {}, dict(y=S + 384, y_stride=256, dim=32, out_stride=96),      # y in the gaps between the rows
+    dict(y=S + 3 * 512 + 384), dict(y=S - 3 * 192 - 192),          # right behind, right before
+    dict(sum=S + 4 * 512), dict(gate=S + 384, gate_stride=128, dim=32), dict(weight=S + 3 * 512 + 384),
+    dict(out=S + 384, out_stride=512), dict(x_type=1, y=S, y_stride=128),
+    dict(x=P + (1 << 17))])
+def test_add_norm_c_takes_memory_apart(change):
+    """Side by side, interleaved, in place: past the checks of the addresses,
+    to the next one, of the scales (so that nothing is launched)."""
+    from vidax_b200 import fp8
+    rc, msg = _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, **IN_PLACE, "out_scale": None, **change}))
+    assert rc == 1 and "out_scale" in msg
+
+
+def test_add_norm_c_overlap_is_byte_for_byte():
+    """Random rows against the sets of bytes they are."""
+    import random
+    from vidax_b200 import fp8
+    rng = random.Random(7)
+    seen = [0, 0]
+    for _ in range(1500):
+        rows, dim = rng.randint(1, 5), rng.randint(1, 6)
+        ss, ys = dim + rng.randint(0, 30), dim + rng.choice([0, rng.randint(0, 60), dim * 3])
+        if rng.random() < 0.3:
+            ys = 2 * ss
+        y = S + 2 * rng.randint(-60, 140)
+        a = _args(fp8.AddNormArgs, **{**NOK, "x": S, "sum": S, "x_stride": ss, "sum_stride": ss, "y": y,
+                                      "y_stride": ys, "out": P + (1 << 19), "out_stride": dim, "rows": rows,
+                                      "rows_per_batch": rows, "dim": dim, "out_scale": None})
+        sum_bytes = {S + r * ss * 4 + i for r in range(rows) for i in range(4 * dim)}
+        meets = any(y + r * ys * 2 + i in sum_bytes for r in range(rows) for i in range(2 * dim))
+        rc, msg = _rc("vx_add_norm", a)
+        assert rc == 1 and ("apart" in msg) == meets, (rows, dim, ss, ys, y - S)
+        seen[meets] += 1
+    assert min(seen) > 200

@@ -275,6 +275,43 @@ def test_add_norm_refuses_overlapping_sums():
         vx.add_norm(buf[:4], y, weight=torch.ones(63, device="cuda"))
 
 
+def test_add_norm_refuses_what_it_would_overwrite_in_place():
+    """residual_out=x: y and the vectors are compared with it too."""
+    import vidax_b200 as vx
+    buf = torch.randn((9, 64), generator=_gen(16), device="cuda")
+    h = buf.bfloat16()
+    y = torch.zeros((8, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="apart"):
+        vx.add_norm(h[1:], h[:-1], residual_out=h[1:])
+    for x in (buf[1:], buf[:8]):
+        for name in ("weight", "bias"):
+            with pytest.raises(ValueError, match="apart"):
+                vx.add_norm(x, y, residual_out=x, **{name: buf[3]})
+        for name in ("gate", "scale", "shift"):
+            with pytest.raises(ValueError, match="apart"):
+                vx.add_norm(x, y, residual_out=x, **{name: buf[3:4]})
+            with pytest.raises(ValueError, match="apart"):
+                vx.add_norm(x.clone(), y, residual_out=x, **{name: buf[3:4]})
+    assert torch.equal(buf.bfloat16(), h)
+    with pytest.raises(TypeError, match="residual_out"):
+        vx.add_norm(x, y, residual_out=[1])
+
+
+def test_add_norm_in_place_on_columns_of_one_buffer():
+    """x and y side by side in a wider buffer, y = x itself, and a copied x."""
+    import vidax_b200 as vx
+    wide = torch.randn((40, 3 * 128), generator=_gen(17), device="cuda").bfloat16()
+    x, y = wide[:, :128], wide[:, 128:256]
+    o, t = vx.add_norm(x.clone(), y.clone(), norm="layer")
+    rest = wide[:, 128:].clone()
+    o2, t2 = vx.add_norm(x, y, norm="layer", residual_out=x)
+    assert t2 is x and torch.equal(x, t) and torch.equal(o2, o) and torch.equal(wide[:, 128:], rest)
+    o, t = vx.add_norm(y.clone(), y.clone())
+    o2, t2 = vx.add_norm(y, y, residual_out=y)
+    assert torch.equal(t2, t) and torch.equal(o2, o)
+    _ok()
+
+
 def test_add_norm_many_batch_items_of_one_row():
     """A CTA's run of rows crosses a batch item at every row."""
     import vidax_b200 as vx

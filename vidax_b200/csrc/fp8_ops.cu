@@ -53,6 +53,35 @@ int check_scale(const char* name, const void* p, const int64_t (&st)[2]) {
   return VX_OK;
 }
 
+// Memory that a call touches: rows of `width` bytes, `stride` bytes apart.
+struct Rows {
+  uintptr_t p;
+  int64_t stride, rows, width;
+  Rows(const void* ptr, int64_t n, int64_t elems_between, int64_t elems, int64_t elem)
+      : p(reinterpret_cast<uintptr_t>(ptr)), stride(elems_between * elem), rows(n), width(elems * elem) {
+    if (rows == 1 || stride == 0) rows = 1, stride = width;  // (vectors may repeat)
+  }
+  bool same(const Rows& o) const { return p == o.p && rows == o.rows && (rows == 1 || stride == o.stride); }
+  uintptr_t end() const { return p + (rows - 1) * stride + width; }
+  // Whether a byte of one is a byte of the other.
+  bool meets(const Rows& o) const {
+    if (end() <= o.p || o.end() <= p) return false;
+    if (rows > 1 && stride == o.stride) {  // columns of one buffer, side by side
+      const int64_t d = static_cast<int64_t>(o.p - p) % stride, at = d < 0 ? d + stride : d;
+      if (at >= width && at + o.width <= stride) return false;
+    }
+    const Rows& a = rows < o.rows ? o : *this;
+    const Rows& b = rows < o.rows ? *this : o;  // the fewer rows
+    for (int64_t i = 0; i < b.rows; ++i) {
+      // the last row of `a` that begins before this row's end
+      const int64_t from = static_cast<int64_t>(b.p - a.p) + i * b.stride, to = from + b.width;
+      if (to <= 0) continue;
+      if (std::min((to - 1) / a.stride, a.rows - 1) * a.stride + a.width > from) return true;
+    }
+    return false;
+  }
+};
+
 // Rows of 8 k elements on 16-byte boundaries (8-byte ones of 1-byte elements).
 bool vec8(const void* p, int64_t stride, int elem) {
   const int64_t bytes = std::min(8 * elem, 16);
@@ -304,12 +333,32 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
     if (vst[i] < 0) return fail(VX_EINVAL, "%s has a negative stride", names[i]);
     if (a->dim > 16384) vec = vec && vec8(vs[i], vst[i], 4);  // the others go through shared memory
   }
+  if (a->rows > INT_MAX) return fail(VX_EUNSUPPORTED, "too many rows");
+  // What is written while other rows are still read lies apart from them. In
+  // place (the sum's rows are x's own) each lane has read what it writes.
+  const Rows x_rows(a->x, a->rows, a->x_stride, a->dim, xe);
+  const Rows y_rows(a->y, a->rows, a->y_stride, a->dim, 2);
+  const Rows sum_rows(a->sum, a->rows, a->sum_stride, a->dim, xe);
+  const Rows out_rows(a->out, a->rows, a->out_stride, a->dim, oe);
+  const bool in_place = a->y != nullptr && sum_rows.same(x_rows);
+  if (out_rows.meets(x_rows) ||
+      (a->y != nullptr && (out_rows.meets(y_rows) || out_rows.meets(sum_rows))))
+    return fail(VX_EINVAL, "out must lie apart from x, y and sum");
+  if (a->y != nullptr && !in_place && sum_rows.meets(x_rows))
+    return fail(VX_EINVAL, "sum must be x itself or lie apart from x");
+  if (a->y != nullptr && !(in_place && y_rows.same(sum_rows) && xe == 2) && sum_rows.meets(y_rows))
+    return fail(VX_EINVAL, "sum must lie apart from y");
+  for (int i = 0; i < 5; ++i) {
+    if (vs[i] == nullptr) continue;
+    const Rows v(vs[i], i < 3 ? a->rows / a->rows_per_batch : 1, vst[i], a->dim, 4);
+    if (out_rows.meets(v) || (a->y != nullptr && sum_rows.meets(v)))
+      return fail(VX_EINVAL, "sum and out must lie apart from %s", names[i]);
+  }
   if (a->out_type == VX_TYPE_E4M3 &&
       (rc = check_scale("out_scale", a->out_scale, a->out_scale_stride)) != VX_OK)
     return rc;
   int dev, sms;
   if ((rc = vx_internal_device(&dev, &sms)) != VX_OK) return rc;
-  if (a->rows > INT_MAX) return fail(VX_EUNSUPPORTED, "too many rows");
   AddNormParams p{};
   p.x = a->x;
   p.sum = a->y != nullptr ? a->sum : nullptr;
