@@ -412,6 +412,40 @@ def test_linear_gelu(m, n, k, out):
     _check_linear(x, w, bias, True, got)
 
 
+@pytest.mark.parametrize("variant", [1, 2, 3, 4])
+def test_linear_gelu_far_from_zero(variant):
+    """Pre-activations of any size (zero products, so each is its bias): the
+    function goes to 0 below and to x above; a NaN stays in its column. At and
+    below -7.5 the function's value is less than 7.5 * 2^-60, and what is
+    computed there is that of -7.5: together below 2^-56."""
+    import vidax_b200 as vx
+    inf, nan = float("inf"), float("nan")
+    b = torch.tensor([-7.4, -7.5, -8.0, -20.0, -1e4, -1e10, -1e19, -2e19, -1e20, -1e30, -3.4e38, -inf, 3.0,
+                      nan, 1.0, 0.0, -0.5, nan, nan, 7.0, 40.0, 1e19, 1e20, 3.4e38, 1.5, inf, -1e25, 2.0])
+    n = b.numel()
+    x = vx.quantize_fp8(torch.zeros((3, 128), device="cuda"))
+    w = vx.quantize_fp8(torch.zeros((n, 128), device="cuda"), 128)
+    y = _f64(vx.linear_fp8(x, w, b.cuda(), activation="gelu_tanh", out_dtype=torch.float32, variant=variant))
+    _ok()
+    v = b.double().numpy()
+    assert (np.isnan(y) == np.isnan(v)).all() and (y == y[:1])[:, ~np.isnan(v)].all()
+    low = v <= -7.5
+    assert (np.abs(y[:, low]) <= 2.0 ** -56).all()
+    assert (y[:, v == inf] == inf).all()
+    mid = ~low & np.isfinite(v)
+    # 0.5 x (1 + tanh u) without the cancellation that leaves 0 of it at -7.4
+    with np.errstate(over="ignore"):
+        want = v[mid] / (1 + np.exp(-2 * np.sqrt(2 / np.pi) * (v[mid] + 0.044715 * v[mid] ** 3)))
+    t = np.minimum(2.31 * np.abs(v[mid]) * (1 + 0.0448 * v[mid] ** 2), 61)
+    assert (np.abs(y[:, mid] - want) <= (7 * U32 * t + 2.0 ** -19) * np.abs(want)).all()
+    if variant < 3:
+        # a large negative pre-activation does not set its block's scale
+        c = torch.where(b < -7, b, 0.25).nan_to_num(0.25, 0.25, -3e38).cuda()
+        q = vx.linear_fp8(x, w, c, activation="gelu_tanh", out_dtype=torch.float8_e4m3fn, variant=variant)
+        _ok()
+        _check_blocks(q, np.repeat(fp8_ref.gelu_tanh(_f64(c).clip(-30))[None], 3, 0), err=2.0 ** -20)
+
+
 @pytest.mark.parametrize("variant", [1, 2, 3])
 @pytest.mark.parametrize("m,n,k", [(1, 40, 100), (128, 64, 128), (300, 700, 1000), (2100, 1300, 512)])
 def test_linear_every_variant(m, n, k, variant):

@@ -181,19 +181,25 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN if either is one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // x / (1 + exp(-2 u)) = 0.5 x (1 + tanh u), u = sqrt(2 / pi) (x + 0.044715 x^3).
 // Two elements share one reciprocal, 1/a = b / (a b): the special-function
-// unit bounds this step. The exponent is bounded so that the product of the
-// denominators stays finite: past 2^60 the quotient is below x * 2^-60, as
-// good as 0.
+// unit bounds this step. So that the product of the denominators stays finite,
+// x counts as -7.5 where it is less: the denominator is 2^60.7 there and the
+// value within 2^-57 of the function's, which goes to 0. The exponent's bound
+// keeps a NaN out of its neighbour's reciprocal.
 __device__ __forceinline__ void gelu_tanh2(float& x, float& y) {
   constexpr float kA = -2.f * 0.7978845608028654f * 1.4426950408889634f;
-  const uint64_t v = f2_pack(x, y);
+  const uint64_t v = f2_pack(max_nan(x, -7.5f), max_nan(y, -7.5f));
   const uint64_t t = f2_mul(
       v, f2_fma(f2_mul(v, v), f2_pack(kA * 0.044715f, kA * 0.044715f), f2_pack(kA, kA)));
   float t0, t1, a, b;
   f2_unpack(t, t0, t1);
-  f2_unpack(f2_add(f2_pack(ex2_approx(fminf(t0, 60.f)), ex2_approx(fminf(t1, 60.f))),
+  f2_unpack(f2_add(f2_pack(ex2_approx(fminf(t0, 61.f)), ex2_approx(fminf(t1, 61.f))),
                    f2_pack(1.f, 1.f)),
             a, b);
   const float r = rcp_approx(a * b);
