@@ -241,3 +241,12 @@ def test_add_norm_c_overlap_is_byte_for_byte():
         assert rc == 1 and ("apart" in msg) == meets, (rows, dim, ss, ys, y - S)
         seen[meets] += 1
     assert min(seen) > 200
+
+
+def test_sizes_past_32_bits_are_refused():
+    from vidax_b200.fp8 import _FLT_MAX, _check_sizes
+    _check_sizes(2 ** 31 - 1, 2 ** 31 - 1)
+    for sizes in ((2 ** 31, 1), (1, 2 ** 31), (1, 1, 2 ** 31)):
+        with pytest.raises(NotImplementedError, match="2\\^31 - 1"):
+            _check_sizes(*sizes)
+    assert _FLT_MAX == float(np.finfo(np.float32).max)

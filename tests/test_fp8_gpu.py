@@ -659,6 +659,36 @@ def test_offsets_past_32_bits():
         del y, ref
 
 
+def test_sizes_past_32_bits_are_refused_by_every_operator():
+    """Views of one element, so nothing of that size exists: an error with a
+    message, before anything is allocated."""
+    import vidax_b200 as vx
+    many = 2 ** 31
+    one = torch.zeros(1, device="cuda")
+    codes = one.to(torch.float8_e4m3fn)
+    w = vx.quantize_fp8(torch.zeros((4, 1), device="cuda"), 128)
+    held = torch.cuda.memory_allocated()
+    for shape in ((many, 1), (1, many), (2, many // 2, 1)):
+        big = one.expand(shape)
+        for call in (lambda: vx.quantize_fp8(big), lambda: vx.add_norm(big)):
+            with pytest.raises(NotImplementedError, match="2\\^31 - 1"):
+                call()
+    x = vx.Fp8Tensor(codes.expand(many, 1), one.expand(many, 1))
+    with pytest.raises(NotImplementedError, match="2\\^31 - 1"):
+        vx.linear_fp8(x, w)
+    x = vx.Fp8Tensor(codes.expand(1, many), one.expand(1, many // 128))
+    with pytest.raises(NotImplementedError, match="2\\^31 - 1"):
+        vx.linear_fp8(x, vx.Fp8Tensor(codes.expand(1, many), one.expand(1, many // 128)))
+    assert torch.cuda.memory_allocated() == held
+    for eps in (-1.0, 1e39, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            vx.add_norm(torch.zeros((2, 8), device="cuda"), eps=eps)
+    x = vx.quantize_fp8(torch.zeros((4, 1), device="cuda"))
+    for variant in (-1, 5, 2 ** 40, None):
+        with pytest.raises(ValueError, match="variant"):
+            vx.linear_fp8(x, w, variant=variant)
+
+
 # ------------------------------------------------------------------ together
 
 

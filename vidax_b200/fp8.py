@@ -157,6 +157,16 @@ def _check_cuda(name: str, t, dtypes, min_dim: int = 1) -> None:
         raise NotImplementedError(f"{name} requires a gradient: this operator is inference only")
 
 
+_INT_MAX = 2 ** 31 - 1
+_FLT_MAX = (2 - 2 ** -23) * 2.0 ** 127
+
+
+def _check_sizes(rows: int, *dims: int) -> None:
+    """What the entry points' 32-bit sizes hold."""
+    if rows > _INT_MAX or max(dims) > _INT_MAX:
+        raise NotImplementedError(f"sizes {(rows, *dims)}: up to 2^31 - 1 rows and features are built")
+
+
 def _row_stride(t: torch.Tensor) -> Optional[int]:
     """Elements between the consecutive rows (..., K) -> (rows, K) of `t`
     without a copy, or None where they are not evenly spaced."""
@@ -219,6 +229,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
         raise ValueError("x has no features")
     dev = x.device
     rows, k = math.prod(x.shape[:-1]), x.shape[-1]
+    _check_sizes(rows, k)
     out, ld, ls = _empty_fp8(x.shape, dev)
     rs = 1
     if block_rows == BLOCK:
@@ -289,12 +300,13 @@ def add_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
         raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
     if out_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
         raise NotImplementedError(f"out_dtype {out_dtype}: bfloat16 and float8_e4m3fn are built")
-    if not eps >= 0:
-        raise ValueError(f"eps must be >= 0, got {eps}")
+    if not 0 <= eps <= _FLT_MAX:
+        raise ValueError(f"eps must be >= 0 and finite in float32, got {eps}")
     dim = x.shape[-1]
     batch = x.shape[0] if x.dim() == 3 else 1
     if dim < 1:
         raise ValueError("x has no features")
+    _check_sizes(batch * x.shape[-2], dim)
     if y is None:
         if gate is not None or residual_out is not None:
             raise ValueError("gate and residual_out belong to y")
@@ -396,9 +408,12 @@ def linear_fp8(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
         raise NotImplementedError(f"activation {activation!r}: None and 'gelu_tanh' are built")
     if out_dtype not in _TYPES:
         raise NotImplementedError(f"out_dtype {out_dtype}: bfloat16, float32 and float8_e4m3fn are built")
-    bp, _, _bias = _vector("bias", bias, (N,), dev)
+    if variant not in range(5):
+        raise ValueError(f"variant must be 0 to 4, got {variant!r}")
     shape = (*xd.shape[:-1], N)
     m = math.prod(shape[:-1])
+    _check_sizes(m, N, K)
+    bp, _, _bias = _vector("bias", bias, (N,), dev)
     if out_dtype == torch.float8_e4m3fn:
         out, ld, ls = _empty_fp8(shape, dev)
         o, os = out.data.data_ptr(), out.scale.data_ptr()
@@ -413,7 +428,7 @@ def linear_fp8(x: Fp8Tensor, w: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
         xs = xs.flatten(0, -2)
     _launch("vx_linear_fp8", dev, xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), ws.data_ptr(), bp, o,
             os, x_stride, w_stride, ld, *xs.stride(), *ws.stride(), 1, ls, m, N, K,
-            _TYPES[out_dtype], _ACTS[activation], variant)
+            _TYPES[out_dtype], _ACTS[activation], int(variant))
     return out
 
 
