@@ -93,3 +93,24 @@ def test_wan_dit_orchestration_matches_oracle(head_dim, batch, monkeypatch):
     assert got.shape == ref.shape == (batch, 2, 8, 16, cfg.out_dim)
     rel = float(np.linalg.norm(got - ref) / np.linalg.norm(ref))
     assert rel <= 2e-2, rel
+
+
+def test_wan_dit_without_blocks():
+    """num_layers = 0: embedding, head and unpatchify alone."""
+    from oracle.wan_dit_ref import wan_dit_forward as ref_forward
+    from vidax_b200 import wan_dit
+    from vidax_b200.prologue import rope3d_freqs
+    cfg = wan_dit.WanConfig(dim=64, ffn_dim=256, num_heads=2, num_layers=0, in_dim=4, out_dim=4,
+                            freq_dim=32, text_dim=64, text_len=16)
+    p = wan_dit.init_params(cfg, "cpu", seed=3)
+    rng = np.random.Generator(np.random.PCG64(6))
+    latents = to_bf16(rng.standard_normal((1, 2, 8, 16, cfg.in_dim)).astype(np.float32))
+    context = to_bf16(rng.standard_normal((1, 10, cfg.text_dim)).astype(np.float32))
+    t = np.array([500.0], np.float32)
+    cos, sin = rope3d_freqs(2, 4, 8, cfg.head_dim)
+    ref = ref_forward(p, cfg, latents, t, context, cos.numpy(), sin.numpy())
+    for q in (p, wan_dit.quantize_params(p, cfg)):
+        got = wan_dit.wan_dit_forward(q, cfg, torch.from_numpy(latents), torch.from_numpy(t),
+                                      torch.from_numpy(context)).float().numpy()
+        assert got.shape == ref.shape
+        assert float(np.linalg.norm(got - ref) / np.linalg.norm(ref)) <= 2e-2

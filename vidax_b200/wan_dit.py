@@ -346,7 +346,7 @@ def wan_dit_forward(p, cfg: WanConfig, latents: torch.Tensor, t: torch.Tensor,
         tp, hp, wp = (latents.shape[1 + i] // cfg.patch_size[i] for i in range(3))
         rope = rope3d_freqs(tp, hp, wp, cfg.head_dim, device=latents.device)
     x, ctx, e0, rope_l, e, grid = pre_process(p, cfg, latents, t, context, rope, sp_axis_name)
-    if isinstance(p["blocks_0.ffn_0_w"], Fp8Tensor):
+    if isinstance(p.get("blocks_0.ffn_0_w"), Fp8Tensor):
         ctx, pending = quantize_fp8(ctx), (None, None)
         for i in range(cfg.num_layers):
             x, pending = _block_forward_fp8(p, i, cfg, x, pending, ctx, e0, rope_l, sp_axis_name)
