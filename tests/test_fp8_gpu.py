@@ -312,6 +312,31 @@ def test_add_norm_in_place_on_columns_of_one_buffer():
     _ok()
 
 
+@pytest.mark.parametrize("stream", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("dim", [129, 300, 768, 1187, 1536, 2500, 4091, 5120, 8000, 13824, 16392, 20001])
+def test_add_norm_in_place_is_the_same(dim, rows, stream):
+    """Every variant by width and row count with residual_out=x, on rows that
+    lie densely and in a wider buffer off the 16-byte boundaries (which may be
+    another variant, with its own order of sums): bit for bit what the same rows
+    give into a new tensor, and nothing around the rows touched."""
+    import vidax_b200 as vx
+    c = _norm_case(1, rows, dim, stream, dim + rows)
+    for out in (torch.float8_e4m3fn, torch.bfloat16):
+        wide = torch.full((rows, dim + 3), 9.0, dtype=stream, device="cuda")
+        for x in (torch.empty_like(c["x"]), wide[None, :, 1:1 + dim]):
+            x.copy_(c["x"])
+            o, total = vx.add_norm(**dict(c, x=x), norm="layer", out_dtype=out)
+            if rows == 3:
+                _check_norm(c, "layer", o, total)
+            o2, t2 = vx.add_norm(**dict(c, x=x), norm="layer", out_dtype=out, residual_out=x)
+            _ok()
+            assert t2 is x and torch.equal(x, total)
+            for a, b in zip(o if isinstance(o, tuple) else (o,), o2 if isinstance(o2, tuple) else (o2,)):
+                assert torch.equal(a.float(), b.float())
+        assert (wide[:, 0] == 9).all() and (wide[:, 1 + dim:] == 9).all()
+
+
 def test_add_norm_many_batch_items_of_one_row():
     """A CTA's run of rows crosses a batch item at every row."""
     import vidax_b200 as vx

@@ -128,3 +128,29 @@ def test_wan_dit_fp8_replays_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("head_dim,batch,P", [(128, 1, 2), (64, 2, 2), (64, 1, 4)])
+def test_wan_dit_fp8_sequence_parallel(head_dim, batch, P, monkeypatch):
+    """Every rank's token chunk through the 8-bit blocks, the ranks emulated as
+    threads: equal to the single-GPU step but for the order of sums (2e-2 as
+    above; a row is normalised and quantised by itself on either side)."""
+    import vidax_b200 as vx
+    from emulated_ranks import RankGroup, run_ranks
+    from vidax_b200 import _lib, ulysses, wan_dit
+    cfg = _tiny(head_dim)
+    q = wan_dit.quantize_params(wan_dit.init_params(cfg, "cuda", seed=3), cfg)
+    single = _run(q, cfg, 5, batch)
+    lat, ctx, t = (torch.from_numpy(x).cuda() for x in _inputs(cfg, 5, batch))
+    fake = RankGroup(P)
+    monkeypatch.setattr(ulysses, "dist", fake)
+    monkeypatch.setattr(wan_dit, "dist", fake)
+    vx.register_axis("sp_fp8", None)
+    try:
+        outs = run_ranks(P, fake, lambda r: wan_dit.wan_dit_forward(
+            q, cfg, lat, t, ctx, sp_axis_name="sp_fp8").float().cpu().numpy())
+    finally:
+        vx.unregister_axis("sp_fp8")
+    assert _lib.device_status() == 0
+    for o in outs:
+        assert o.shape == single.shape and _rel(o, single) <= 2e-2, _rel(o, single)
