@@ -245,8 +245,23 @@ def test_add_norm_c_overlap_is_byte_for_byte():
 
 def test_sizes_past_32_bits_are_refused():
     from vidax_b200.fp8 import _FLT_MAX, _check_sizes
-    _check_sizes(2 ** 31 - 1, 2 ** 31 - 1)
-    for sizes in ((2 ** 31, 1), (1, 2 ** 31), (1, 1, 2 ** 31)):
+    _check_sizes(2 ** 31 - 1, 2 ** 31 - 4096)
+    for sizes in ((2 ** 31, 1), (1, 2 ** 31), (1, 1, 2 ** 31), (1, 2 ** 31 - 4095)):
         with pytest.raises(NotImplementedError, match="2\\^31 - 1"):
             _check_sizes(*sizes)
     assert _FLT_MAX == float(np.finfo(np.float32).max)
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31 - 256, 2 ** 31 - 2000])
+def test_features_whose_indices_would_overflow_are_refused(most):
+    """The kernels step past a row's end by up to 2048 features in 32 bits; one
+    that wrapped would read at a negative offset. Refused before a launch."""
+    from vidax_b200 import fp8
+    far = dict(x_stride=2 ** 31, out_stride=2 ** 31, y=None, sum=None)
+    for rows in (1, 4):
+        rc, msg = _rc("vx_add_norm", _args(fp8.AddNormArgs, **{**NOK, **far, "rows": rows, "rows_per_batch": 1,
+                                                              "dim": most}))
+        assert rc == 2 and "features" in msg
+    for change in (dict(n=most, out_stride=2 ** 31), dict(k=most, x_stride=2 ** 31, w_stride=2 ** 31)):
+        rc, msg = _rc("vx_linear_fp8", _args(fp8.LinearFp8Args, **{**LOK, **change}))
+        assert rc == 2 and "features" in msg

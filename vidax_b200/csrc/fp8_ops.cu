@@ -26,6 +26,10 @@ int fail(int code, const char* fmt, A... a) {
 }
 int fail(int code, const char* msg) { return vx_internal_fail(code, msg); }
 
+// Features that the kernels' 32-bit feature indices can step past the end of: a
+// step is up to 2048 of them.
+constexpr int32_t kMostFeatures = INT_MAX - 4095;
+
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int launched(const char* what) {
@@ -333,7 +337,8 @@ extern "C" int vx_add_norm(const vx_add_norm_args* a, vx_stream_t stream) {
     if (vst[i] < 0) return fail(VX_EINVAL, "%s has a negative stride", names[i]);
     if (a->dim > 16384) vec = vec && vec8(vs[i], vst[i], 4);  // the others go through shared memory
   }
-  if (a->rows > INT_MAX) return fail(VX_EUNSUPPORTED, "too many rows");
+  if (a->rows > INT_MAX || a->dim > kMostFeatures)
+    return fail(VX_EUNSUPPORTED, "too many rows or features (%lld x %d)", (long long)a->rows, a->dim);
   // What is written while other rows are still read lies apart from them. In
   // place (the sum's rows are x's own) each lane has read what it writes.
   const Rows x_rows(a->x, a->rows, a->x_stride, a->dim, xe);
@@ -409,6 +414,8 @@ int linear_call(const vx_linear_fp8_args* a, const LinTest* test, vx_stream_t st
   if (a == nullptr) return fail(VX_EINVAL, "args is NULL");
   if (a->m < 0 || a->n < 1 || a->k < 1)
     return fail(VX_EINVAL, "bad sizes (m %d, n %d, k %d)", a->m, a->n, a->k);
+  if (a->n > kMostFeatures || a->k > kMostFeatures)
+    return fail(VX_EUNSUPPORTED, "too many features (n %d, k %d)", a->n, a->k);
   const int out_idx = a->out_type == VX_TYPE_BF16    ? kOutBf16
                       : a->out_type == VX_TYPE_FLOAT ? kOutFloat
                       : a->out_type == VX_TYPE_E4M3  ? kOutE4m3

@@ -162,9 +162,9 @@ _FLT_MAX = (2 - 2 ** -23) * 2.0 ** 127
 
 
 def _check_sizes(rows: int, *dims: int) -> None:
-    """What the entry points' 32-bit sizes hold."""
-    if rows > _INT_MAX or max(dims) > _INT_MAX:
-        raise NotImplementedError(f"sizes {(rows, *dims)}: up to 2^31 - 1 rows and features are built")
+    """What the entry points' 32-bit sizes hold, and their indices past a row's end."""
+    if rows > _INT_MAX or max(dims) > _INT_MAX - 4095:
+        raise NotImplementedError(f"sizes {(rows, *dims)}: up to 2^31 - 1 rows of 2^31 - 4096 features are built")
 
 
 def _row_stride(t: torch.Tensor) -> Optional[int]:
