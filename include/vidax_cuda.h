@@ -406,7 +406,11 @@ int vx_gated_residual(float* x, const void* y, const float* gate, int64_t rows, 
  * A NaN stays a NaN in its place; a block with an infinity gets s = inf and
  * stands for NaN. Scales are addressed by two element strides, {row (block),
  * feature block}; the kernels prefer row stride 1. Rows are addressed by an
- * element stride; nothing behind a row's `dim` elements is read or written.
+ * element stride. Nothing outside a row's `dim` elements is written, or has a
+ * part in a result; loads may take in the rest of the aligned 16 bytes that a
+ * row begins or ends in (up to 15 bytes before and behind it, the first and the
+ * last row's too). What a call writes lies apart from what it reads, except
+ * where an entry point says otherwise.
  */
 enum { VX_TYPE_FLOAT = 0, VX_TYPE_BF16 = 1, VX_TYPE_E4M3 = 2 };
 enum { VX_NORM_RMS = 0, VX_NORM_LAYER = 1 };

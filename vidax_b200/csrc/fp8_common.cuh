@@ -53,8 +53,8 @@ __device__ __forceinline__ float lanes_max(float m) {
 // on 16-byte boundaries. Any other row (odd widths or strides) is read through
 // the aligned 16-byte pieces that its bytes lie in, shifted into place: a row
 // starts at another offset each time, but the same for all lanes. A piece that
-// holds one of the row's bytes lies in the same page, so nothing outside the
-// caller's memory is touched that could fault.
+// holds one of the row's bytes lies in the same page, so the up to 15 bytes of
+// it before the first row or behind the last cannot fault.
 
 // The lane's eight elements as they lie in memory (`row` points at the chunk,
 // of which the first `n` features exist; the others read 0).

@@ -24,7 +24,7 @@
 // tensor map clips at the next one and up to 15 bytes behind the row would be
 // written.
 //
-// What bounds it, measured on 9472 x 8960 -> 2048 (177-184 us, 1930 TFLOP/s, a
+// What bounds it, measured on 9472 x 8960 -> 2048 (171-188 us, 1930 TFLOP/s, a
 // plain e4m3 product of the library 131 us): the power cap (1000 W, at 1425 of
 // 1965 MHz). Of the time, adding the scaled products is some 30 us and reading
 // them from TMEM 10. A block takes 920 cycles, 512 of them MMAs; the rest is

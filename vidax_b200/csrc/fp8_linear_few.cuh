@@ -52,7 +52,8 @@ __device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint3
 }
 
 // 16 bytes at feature k0 of a row; those at k and after are 0 (what lies there
-// may be anything, a NaN times 0 too).
+// may be anything, a NaN times 0 too, and in the last row behind the tensor: the
+// 16 bytes are aligned, so the row's own ones are in the same page).
 __device__ __forceinline__ uint4 few_load(const uint8_t* row, int k0, int k) {
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   if (k0 < k) {

@@ -144,8 +144,10 @@ int launch_add_norm(AddNormParams& p, int dev, int sms, cudaStream_t s) {
     if (vecs <= 4) return launch_norm<T, 1, 4, kVec>(p, dev, sms, s);
     if constexpr (kVec) return launch_norm<T, 1, 6, kVec>(p, dev, sms, s);
   }
-  // (5 or 6 chunks: two warps with three each, 32760 x 1187 10 % faster than
-  // four of which some hold two)
+  // (5 or 6 chunks: two warps with three each against four of which some hold
+  // two, rows of 1027, 1283 and 1533 features in us, bf16 stream: 700 rows 7.0 /
+  // 7.8, 7.4 / 8.6, 7.8 / 8.6; 4678 rows 18.0 / 21.7, 19.7 / 23.4, 20.5 / 24.2;
+  // 32760 rows 118 / 133, 128 / 145, 134 / 149)
   if constexpr (!kVec) {
     if (!few && vecs > 4 && vecs <= 6) return launch_norm<T, 2, 3, kVec>(p, dev, sms, s);
   }
@@ -190,7 +192,12 @@ LinVariant variant(double block, double tile) {
 }
 
 // Measured: 9472 x 8960 -> 2048 takes 922 / 566 / 425 cycles per block, and a
-// tile's start and output 2500 / 2000 / 2000 besides.
+// tile's start and output 2500 / 2000 / 2000 besides. With GELU and an e4m3
+// output a tile's end is longer, by about as much for every column, so the same
+// model serves. Its choice against the best of the tiles, 16 products of 64 to
+// 32760 rows: with GELU and e4m3 within 2 % (4680 x 1536 -> 8960: 95 us, the
+// 128-column tile 110), with a bf16 output within 3 % from 1500 rows on and within 7 %
+// (0.4 us) below.
 const LinVariant kVariants[] = {variant<256>(922, 2500), variant<128>(566, 2000),
                                 variant<64>(425, 2000)};
 constexpr int kNumVariants = sizeof(kVariants) / sizeof(kVariants[0]);
